@@ -243,9 +243,11 @@ def _plain_plan(s):
     page, q, c = s["case"]["page"], s["query_lens"], s["context_lens"]
     have = (c + page - 1) // page
     need = (c + q + page - 1) // page - have
-    cum = torch.cumsum(need, 0, dtype=torch.int32)
     table = s["table"]
-    granted = ((need == 0) | (cum <= s["free_count"])) & (have + need <= table.shape[1])
+    fits = have + need <= table.shape[1]
+    need = torch.where(fits, need, 0)
+    cum = torch.cumsum(need, 0, dtype=torch.int32)
+    granted = ((need == 0) | (cum <= s["free_count"])) & fits
     at = torch.arange(table.shape[1], device=q.device)[None, :] - have[:, None]
     new = (at >= 0) & (at < need[:, None]) & granted[:, None]
     taken = s["free_count"] - 1 - ((cum - need)[:, None] + at)
