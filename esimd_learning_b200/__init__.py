@@ -32,4 +32,8 @@ from custom_esimd_kernels_vllm.ops import (  # noqa: E402,F401
     esimd_quant_fp8_per_token,
     esimd_set_weight_prefetch,
     esimd_gemm_fp8_pertoken_pern,
+    esimd_kv_plan,
+    esimd_kv4_append,
+    esimd_kv4_gather,
+    esimd_kv4_attention,
 )

@@ -7,8 +7,10 @@ Outputs:
       torch.library registration of the GEMV / add+RMSNorm / decode-helper ops (g++)
   python/custom_esimd_kernels_vllm/custom_esimd_kernels_gemm.so
       torch.library registration of the GEMM ops
+  python/custom_esimd_kernels_vllm/custom_esimd_kernels_kv4.so
+      torch.library registration of the paged 4-bit key/value cache ops
 
-The two extension modules keep the reference's module names and PyInit
+The first two extension modules keep the reference's module names and PyInit
 symbols (csrc/xpu/torch_extension.cc:21-24, torch_extension_gemm.cc:16-20) and
 sit in the reference's wrapper package, so
 `from custom_esimd_kernels_vllm import custom_esimd_kernels, custom_esimd_kernels_gemm`
@@ -35,10 +37,12 @@ CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 NVCC = str(CUDA_HOME / "bin" / "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-CU_SOURCES = ["abi.cu", "gemv_fp8.cu", "gemv_fp8_bulk.cu", "rmsnorm.cu", "elementwise.cu", "tp_allreduce.cu", "gemm_fp8_tcgen05.cu"]
+CU_SOURCES = ["abi.cu", "gemv_fp8.cu", "gemv_fp8_bulk.cu", "rmsnorm.cu", "elementwise.cu", "tp_allreduce.cu", "gemm_fp8_tcgen05.cu",
+              "kv4_cache.cu", "kv4_attention.cu"]
 EXT_MODULES = {
     "custom_esimd_kernels": "torch_extension.cc",
     "custom_esimd_kernels_gemm": "torch_extension_gemm.cc",
+    "custom_esimd_kernels_kv4": "torch_extension_kv4.cc",
 }
 LIB_NAME = "libcek_b200.so"
 
@@ -107,7 +111,7 @@ def build_ext(force: bool = False) -> list[Path]:
         if force or _stale(out, [s, lib] + _headers()):
             jobs.append(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", *cflags, str(s), "-o", str(out),
                          f"-L{PKG}", "-l:" + LIB_NAME, "-Wl,-rpath,$ORIGIN/../../esimd_learning_b200", *ldflags])
-    with cf.ThreadPoolExecutor(max_workers=2) as ex:
+    with cf.ThreadPoolExecutor(max_workers=3) as ex:
         list(ex.map(_run, jobs))
     return outs
 

@@ -22,6 +22,7 @@ CEK_E4M3, CEK_E5M2 = 0, 1
 CEK_SCALE_PERN_F16, CEK_SCALE_PERN_F32, CEK_SCALE_PERT_F32 = 0, 1, 2
 CEK_GEMV_EARLY_WEIGHTS = 1
 CEK_GEMV_GELU_MUL_OUTPUT = 2
+CEK_KV_PLAN_MAX_REQUESTS = 4096
 CEK_COMM_SYNC_BYTES = 4096  # data area offset inside a comm region (include/cek.h)
 
 _P = ctypes.c_void_p
@@ -29,6 +30,16 @@ _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
 _U = ctypes.c_uint
+
+
+
+class Kv4Cache(ctypes.Structure):
+    """cek_kv4_cache (include/cek.h)."""
+    _fields_ = [("data", _P), ("scales", _P), ("num_pages", _I64), ("page_stride", _I64), ("head_stride", _I64),
+                ("kv_heads", _I64), ("head_dim", _I64), ("page_size", _I64)]
+
+
+_C = ctypes.POINTER(Kv4Cache)
 
 # name -> (restype, argtypes); must list every function include/cek.h declares.
 SIGNATURES = {
@@ -60,6 +71,12 @@ SIGNATURES = {
     "cek_gemm_fp8w_workspace_bytes": (_I64, [_I64, _I64]),
     "cek_gemm_fp8w": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _I, _P]),
     "cek_gemm_fp8w_preferred": (_I, [_I64, _I64, _I64]),
+    "cek_kv4_page_bytes": (_I64, [_I64, _I64]),
+    "cek_kv_plan": (_I, [_P] * 10 + [_I64] * 6 + [_P]),
+    "cek_kv4_append": (_I, [_P, _P, _P, _C] + [_I64] * 5 + [_I, _P]),
+    "cek_kv4_gather": (_I, [_C, _P, _P, _P] + [_I64] * 5 + [_I, _P]),
+    "cek_kv4_attention_workspace_bytes": (_I64, [_I64] * 7),
+    "cek_kv4_attention": (_I, [_P, _C] + [_P] * 5 + [_I64] * 10 + [_F] + [_I64] * 3 + [_I, _P]),
     "cek_gemv_fp8_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint64)]),
     "cek_gemm_fp8_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint64)]),
 }

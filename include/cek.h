@@ -316,6 +316,114 @@ CEK_API int cek_gemv_fp8_timeouts(uint64_t* count);
  * since the library was loaded (0 in a healthy run).  Synchronous. */
 CEK_API int cek_gemm_fp8_timeouts(uint64_t* count);
 
+/* ---- paged 4-bit key/value cache ------------------------------------------
+ * What the decode chain needs between cek_qkv_norm_rope and its attention
+ * output: page bookkeeping on the device, a cache of keys and values in 4
+ * bits, and attention that reads it.  No reference counterpart.
+ *
+ * data [num_pages, kv_heads, page bytes] uint8; page_size P in {16, 32, 64,
+ * 128} tokens, head_dim D in {64, 128, 256}; one (page, head) block is
+ * cek_kv4_page_bytes(P, D) = P (D + D / 8) contiguous bytes:
+ *   K codes [P, D/2] | K scales [P, D/16] | V codes [P, D/2] | V scales [P, D/16].
+ * A code is an e2m1 number (0, .5, 1, 1.5, 2, 3, 4, 6 and a sign bit),
+ * channel 2i in the low four bits of byte i; a scale is an e4m3 number for 16
+ * channels of one token.  A value stands for code * scale * scales[kv, head]
+ * with `scales` fp32 [2, kv_heads] (keys, then values), positive and finite,
+ * read on the device.  page_stride and head_stride are in bytes, multiples of
+ * 16, at least a block each.  A slot is page * P + offset. */
+typedef struct {
+  void* data;
+  const float* scales;
+  int64_t num_pages, page_stride, head_stride;
+  int64_t kv_heads, head_dim, page_size;
+} cek_kv4_cache;
+/* Bytes of one (page, head) block; 0 for a size that is not supported. */
+CEK_API int64_t cek_kv4_page_bytes(int64_t page_size, int64_t head_dim);
+
+/* ---- page plan of one step, from request lengths ---------------------------
+ * Request i of `requests` brings n_i = query_lens[i] new tokens behind the
+ * c_i = context_lens[i] that its pages hold.  All arrays are int32 on the
+ * device unless said otherwise.
+ *   need_i  = ceil((c_i + n_i) / P) - ceil(c_i / P) pages, taken from the top
+ *             of the stack free_pages[0 .. free_count): request by request,
+ *             the next one is free_pages[free_count - 1 - (pages taken)];
+ *   block_table [requests, table_width] (row stride table_stride elements)
+ *             gets the new pages in its entries [ceil(c_i/P), ceil((c_i+n_i)/P));
+ *   query_start [requests + 1]: exclusive sums of n;  seq_lens[i] = c_i + n_i;
+ *   positions, slot_mapping: int64 [tokens], the position and the slot of
+ *             each new token; entries past the last token get 0 and -1, tokens
+ *             past `tokens` are dropped;
+ *   free_count_out[0]: free pages that are left.
+ * A request that the stack (in order) or its table row cannot serve is refused
+ * whole: it takes no page, its slots are -1 and its seq_lens entry is ~c_i
+ * (negative), which attention reads as an empty request and a later plan
+ * keeps refused.  Negative n count as 0.
+ * seq_lens may be context_lens and free_count_out may be free_count (the state
+ * then advances in place: nothing of them is written before all is read); no
+ * other arrays may overlap.  The sums of n and of need must stay below 2^31.
+ * requests <= CEK_KV_PLAN_MAX_REQUESTS; any page_size >= 1. */
+#define CEK_KV_PLAN_MAX_REQUESTS 4096
+CEK_API int cek_kv_plan(const int32_t* query_lens, const int32_t* context_lens, int32_t* block_table,
+                        const int32_t* free_pages, const int32_t* free_count, int32_t* query_start,
+                        int32_t* seq_lens, int32_t* free_count_out, int64_t* positions,
+                        int64_t* slot_mapping, int64_t requests, int64_t table_width,
+                        int64_t table_stride, int64_t pool_size, int64_t tokens, int64_t page_size,
+                        void* stream);
+
+/* ---- write tokens into the cache -------------------------------------------
+ * key, value: [tokens, kv_heads, head_dim] fp16/bf16 with the given token and
+ * head strides (elements), channels contiguous (views of a qkv tensor).  For
+ * each group of 16 channels, in fp32 with correctly rounded operations:
+ *   s = e4m3(min(max|x| / (6 g), 448)),  code = e2m1(x / (s g)),
+ * both round-to-nearest-even (beyond 6: 6), g the head's kv scale; s g = 0
+ * gives zeros.  A NaN makes its group's scale NaN; infinities saturate.
+ * slot_mapping int64 [tokens]; a token whose slot is negative or beyond the
+ * cache is skipped.  Slots must differ. */
+CEK_API int cek_kv4_append(const void* key, const void* value, const int64_t* slot_mapping,
+                           const cek_kv4_cache* cache, int64_t tokens, int64_t key_token_stride,
+                           int64_t key_head_stride, int64_t value_token_stride,
+                           int64_t value_head_stride, int dtype, void* stream);
+
+/* ---- read tokens back in 16 bits -------------------------------------------
+ * key, value [tokens, kv_heads, head_dim] (strides as above) = the values that
+ * the slots stand for, rounded once from fp32; zeros for a slot that is
+ * negative or beyond the cache.  A slot may be read more than once. */
+CEK_API int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, void* key, void* value,
+                           int64_t tokens, int64_t key_token_stride, int64_t key_head_stride,
+                           int64_t value_token_stride, int64_t value_head_stride, int dtype,
+                           void* stream);
+
+/* ---- attention over the cache ----------------------------------------------
+ * query [tokens, q_heads, head_dim], out the same (token and head strides in
+ * elements, multiples of 8; channels contiguous).  Rows query_start[i] ..
+ * query_start[i+1] belong to request i and are the last n_i of its seq_lens[i]
+ * tokens: row r stands at position p = seq_lens[i] - n_i + r and sees the keys
+ * max(0, p - window + 1) .. p (window 0: all of 0 .. p) of the pages
+ * block_table[i]; query head h reads kv head h / (q_heads / kv_heads).
+ *   out = sum_j softmax_j(softmax_scale q . k_j) v_j
+ * with the sums, maxima and the output accumulated in fp32; probabilities are
+ * rounded to fp16 for the product with the values.  A row that sees no key
+ * (an empty or refused request) gets zeros.  Nothing behind a row's last key
+ * reaches it, NaN included.  Rows past query_start[requests] are not written.
+ * max_query_len and max_seq_len are bounds of n_i and seq_lens[i] known on the
+ * host (a longer request is read as if cut there: its rows past the bound are
+ * not written, its keys past it not read); seq_lens are also cut to
+ * table_width * P.  Page numbers outside the cache are clamped into it.
+ * workspace: cek_kv4_attention_workspace_bytes() bytes, 16-byte aligned,
+ * contents ignored; may be null where that is 0.  One call at a time per
+ * workspace.  Deterministic: no atomics order a sum. */
+CEK_API int64_t cek_kv4_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t q_heads,
+                                                  int64_t kv_heads, int64_t head_dim,
+                                                  int64_t max_query_len, int64_t max_seq_len);
+CEK_API int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, const int32_t* block_table,
+                              const int32_t* query_start, const int32_t* seq_lens, void* out,
+                              void* workspace, int64_t workspace_bytes, int64_t requests,
+                              int64_t tokens, int64_t q_heads, int64_t table_width,
+                              int64_t table_stride, int64_t query_token_stride,
+                              int64_t query_head_stride, int64_t out_token_stride,
+                              int64_t out_head_stride, float softmax_scale, int64_t max_query_len,
+                              int64_t max_seq_len, int64_t window, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,7 +1,7 @@
 """The vLLM custom-op wrapper package, under the reference's own name and
 layout (python/custom_esimd_kernels_vllm/__init__.py:1-13), for NVIDIA B200.
 
-Importing it loads its two torch.library extension modules, which register
+Importing it loads its torch.library extension modules, which register
 the ops in the `torch.ops.custom_esimd_kernels_vllm` namespace on the CUDA
 dispatch key (the kernels live in esimd_learning_b200/libcek_b200.so), and
 re-exports the Python wrappers of `ops`.  A caller of the XPU build keeps its
@@ -17,6 +17,7 @@ import torch  # noqa: F401  (loads libtorch before the extension modules)
 try:
     from custom_esimd_kernels_vllm import custom_esimd_kernels  # noqa: F401
     from custom_esimd_kernels_vllm import custom_esimd_kernels_gemm  # noqa: F401
+    from custom_esimd_kernels_vllm import custom_esimd_kernels_kv4  # noqa: F401
 except ImportError as e:  # pragma: no cover - exercised only on an unbuilt tree
     raise ImportError(
         "custom_esimd_kernels_vllm extensions are not built; run "
@@ -37,4 +38,8 @@ from custom_esimd_kernels_vllm.ops import (  # noqa: E402,F401
     esimd_quant_fp8_per_token,
     esimd_set_weight_prefetch,
     esimd_gemm_fp8_pertoken_pern,
+    esimd_kv_plan,
+    esimd_kv4_append,
+    esimd_kv4_gather,
+    esimd_kv4_attention,
 )

@@ -160,3 +160,73 @@ def esimd_gemm_fp8_pertoken_pern(
     weight e4m3 [N, K] with weight_scale fp32 [N], output fp16/bf16 [M, N].
     K % 128 == 0, N % 16 == 0.  Returns output."""
     return _ops.esimd_gemm_fp8_pertoken_pern(input_q, input_scale, weight, weight_scale, output)
+
+
+def esimd_kv_plan(
+    query_lens: torch.Tensor, context_lens: torch.Tensor, block_table: torch.Tensor,
+    free_pages: torch.Tensor, free_count: torch.Tensor, page_size: int,
+    query_start: torch.Tensor, seq_lens: torch.Tensor, free_count_out: torch.Tensor,
+    positions: torch.Tensor, slot_mapping: torch.Tensor,
+) -> torch.Tensor:
+    """Pages, slots and positions of one step, on the device from request lengths.
+
+    Request i brings query_lens[i] tokens behind the context_lens[i] that its
+    pages hold (int32 [requests], at most 4096).  New pages come from the top of
+    the stack free_pages[:free_count] (int32), request by request, and are
+    written behind the old ones in block_table (int32 [requests, width]).
+    Written: query_start int32 [requests + 1], seq_lens int32 [requests],
+    free_count_out int32 [1], positions and slot_mapping int64 [tokens] (slot =
+    page * page_size + offset; 0 and -1 past the last token).  A request that the
+    stack or its table row cannot serve is refused whole: slots -1, no page, and
+    seq_lens[i] = -context_lens[i] - 1, which attention reads as empty and later
+    plans keep refused.  seq_lens may be context_lens and free_count_out may be
+    free_count: the state then advances in place, as a captured decode step
+    needs.  Returns slot_mapping."""
+    return _ops.esimd_kv_plan(query_lens, context_lens, block_table, free_pages, free_count, page_size,
+                              query_start, seq_lens, free_count_out, positions, slot_mapping)
+
+
+def esimd_kv4_append(
+    key: torch.Tensor, value: torch.Tensor, kv_scales: torch.Tensor, slot_mapping: torch.Tensor,
+    kv_cache: torch.Tensor, page_size: int,
+) -> torch.Tensor:
+    """Quantises tokens into the paged 4-bit cache and returns it.
+
+    key, value [tokens, kv_heads, head_dim] fp16 or bf16, channels contiguous
+    (views of a qkv tensor are fine), head_dim 64, 128 or 256; slot_mapping int64
+    [tokens], all different; a token with a negative slot is skipped.  kv_cache
+    uint8 [pages, kv_heads, page_size * (head_dim + head_dim // 8)], page_size 16,
+    32, 64 or 128: per block K codes, K scales, V codes, V scales.  16 channels
+    share s = e4m3(max|x| / (6 g)) with g = kv_scales[k or v, head] (fp32
+    [2, kv_heads]); a channel is kept as e2m1(x / (s g)), two to a byte."""
+    return _ops.esimd_kv4_append(key, value, kv_scales, slot_mapping, kv_cache, page_size)
+
+
+def esimd_kv4_gather(
+    kv_cache: torch.Tensor, kv_scales: torch.Tensor, slots: torch.Tensor,
+    key: torch.Tensor, value: torch.Tensor, page_size: int,
+):
+    """Reads tokens back in 16 bits: key and value [tokens, kv_heads, head_dim]
+    get the values that the cache holds for `slots` (int64 [tokens]; zeros for a
+    negative one).  Returns (key, value)."""
+    _ops.esimd_kv4_gather(kv_cache, kv_scales, slots, key, value, page_size)
+    return key, value
+
+
+def esimd_kv4_attention(
+    query: torch.Tensor, kv_cache: torch.Tensor, kv_scales: torch.Tensor, block_table: torch.Tensor,
+    query_start: torch.Tensor, seq_lens: torch.Tensor, output: torch.Tensor, page_size: int,
+    softmax_scale: float, max_query_len: int, max_seq_len: int, window: int = 0,
+) -> torch.Tensor:
+    """Causal attention of a step's tokens over the paged 4-bit cache.
+
+    query, output [tokens, q_heads, head_dim] fp16 or bf16 (query may be a view
+    of a qkv tensor); the tokens of request i are rows query_start[i] ..
+    query_start[i + 1], the last ones of its seq_lens[i] tokens, which
+    esimd_kv4_append has written through the same block_table.  A token at
+    position p sees the keys max(0, p - window + 1) .. p (window 0: all);
+    q_heads is a multiple of the cache's kv heads.  A row that sees nothing gets
+    zeros.  max_query_len and max_seq_len bound the step's lengths on the host
+    (they choose the kernel and the workspace).  Returns output."""
+    return _ops.esimd_kv4_attention(query, kv_cache, kv_scales, block_table, query_start, seq_lens, output,
+                                    page_size, softmax_scale, max_query_len, max_seq_len, window)
