@@ -1,9 +1,11 @@
 // kv4_attention.cu — attention over the paged 4-bit key/value cache
 // (cek_kv4_attention).
 #include "kv4.cuh"
+#include "mbarrier.cuh"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace cek {
 namespace kv4 {
@@ -17,8 +19,9 @@ struct AttnParams {
   const int32_t* seq_lens;
   int64_t table_stride, qts, qhs, ots, ohs;
   int requests, tokens, q_heads, group, table_width, P;
-  int max_q, max_seq, window;
+  int max_q, max_seq, key_limit, window;  // key_limit: table_width * P
   float scale_log2;  // softmax_scale * log2(e)
+  float* partial;    // pieces of split segments
 };
 
 // One warp per (token, query head): a lane scores one key of 32, then holds
@@ -101,13 +104,762 @@ attn_simple_kernel(const AttnParams p) {
   for (int e = 0; e < E; ++e) out[lane * E + e] = from_f32<T>(l == 0.f ? 0.f : o[e] / l * vf);
 }
 
+// ---- decode ------------------------------------------------------------------
+// Few rows a request (single tokens, drafted tokens): the cache is read once
+// and HBM is the bound; what has to keep up is turning 4-bit codes into matrix
+// operands.
+//
+//  * A warp is a worker with a ring of its own in shared memory: it asks for
+//    the pages of its next tiles (TK keys; one bulk copy a page, since a
+//    (page, head) block is contiguous) and computes on the oldest one.  No
+//    barrier between warps until the end.
+//  * The tiles of all (request, kv head, row block) segments form one line, cut
+//    into equal ranges, one a worker: ragged lengths cost no idle time.  A
+//    segment inside one range is written out by its worker; the pieces of the
+//    others (running maximum, sum, unnormalised output) go to the workspace and
+//    attn_join_kernel adds them in the order of the keys.
+//  * S^T = K Q^T and O^T = V^T P^T: keys (channels) are the 16 rows of
+//    mma.sync m16n8k16, up to 8 NT query rows its columns, so 8 heads of a
+//    group waste nothing.  Lane (g, t) of a warp reads the codes of key g's
+//    channels [t D/4, (t+1) D/4) in 16 bytes; the order of channels within the
+//    sum is free as long as the query's fragments have the same.
+//  * codes become f16x2 by cvt (two codes), times the group's scale: exact
+//    (kv4.cuh).  A value fragment pairs two keys of one channel: the words of two
+//    keys are interleaved nibble by nibble before the conversion, two
+//    operations for four pairs.
+//  * Key row r of a 16-key block is key (r & 8) + ((r & 7) >> 1) + 4 (r & 1):
+//    then the value lanes of one access read four neighbouring keys.
+//  * The probabilities of a tile, rounded to fp16, turn into the second
+//    product's operand by movmatrix.  They are held as 2^kShift p, so that fp16
+//    keeps full precision down to p = 2^-28.
+//  * bf16 queries are scaled by a power of two a row, exactly, into fp16's
+//    range: one multiply path for both types (what falls out below is 2^-38 of
+//    the row's largest channel).
+constexpr float kShift = 14.f;
+constexpr int kDecodeWarps = 4;
+constexpr int kDecodeThreads = 32 * kDecodeWarps;
+constexpr int kMaxRequests = 2048;  // per launch: their prefix sums sit in shared memory
+constexpr uint32_t kWaitPolls = 1u << 22;
+
+__device__ unsigned long long g_timeouts;
+
+template <int D>
+struct DecodeCfg {
+  static constexpr int TK = D == 256 ? 32 : 64;                 // keys of a tile
+  static constexpr int STAGE = Layout<D>::bytes(TK);
+  static constexpr int STAGES = 3;
+};
+
+// What a request asks for, from its lengths.
+struct Request {
+  int t0, n;          // first token row, rows tokens (bounded)
+  int pos0;           // position of the first token
+  int tile0, tiles;   // tiles of TK keys that any row sees (at least one if n > 0: it writes the zeros)
+  int end;            // keys behind it do not exist
+};
+template <int TK>
+CEK_DEVICE Request request_of(const AttnParams& p, int b) {
+  Request r;
+  r.t0 = p.query_start[b];
+  const int n = max(p.query_start[b + 1] - r.t0, 0);
+  const int seq = p.seq_lens[b];
+  r.n = min(n, p.max_q);
+  r.pos0 = max(seq, 0) - n;  // a refused request (negative): every row stands before position 0
+  r.end = max(0, min(min(r.pos0 + r.n, p.max_seq), p.key_limit));
+  const int lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
+  r.tile0 = min(lo, r.end) / TK;
+  r.tiles = r.n > 0 ? max(1, (r.end + TK - 1) / TK - r.tile0) : 0;
+  return r;
+}
+
+struct Segment {
+  int b, h, rb;
+  Request r;
+  int first, tiles;  // its tiles are [first, first + tiles) of the line
+};
+
+// prefix[b] = tiles of the requests before b, all heads and row blocks
+template <int TK, int ROWS>
+CEK_DEVICE Segment segment_at(const AttnParams& p, const int32_t* prefix, int tile) {
+  int lo = 0, hi = p.requests - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= tile) lo = mid; else hi = mid - 1;
+  }
+  Segment s;
+  s.b = lo;
+  s.r = request_of<TK>(p, lo);
+  s.tiles = s.r.tiles;
+  const int rbs = (s.r.n * p.group + ROWS - 1) / ROWS;
+  const int idx = (tile - prefix[lo]) / s.tiles;
+  s.h = idx / rbs;  // the row blocks of a head side by side: they read the same pages
+  s.rb = idx % rbs;
+  s.first = prefix[lo] + idx * s.tiles;
+  return s;
+}
+
+// Exclusive sums of the requests' tiles into prefix[0 .. requests]; the whole block calls it.
+template <int TK, int ROWS>
+CEK_DEVICE void scan_requests(const AttnParams& p, int32_t* prefix, int32_t* warp_sum) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  int carry = 0;
+  for (int b0 = 0; b0 < p.requests; b0 += blockDim.x) {
+    const int b = b0 + tid;
+    int v = 0;
+    if (b < p.requests) {
+      const Request r = request_of<TK>(p, b);
+      v = r.tiles * p.cache.heads * ((r.n * p.group + ROWS - 1) / ROWS);
+    }
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += a;
+    }
+    if (lane == 31) warp_sum[warp] = s;
+    __syncthreads();
+    int before = carry, all = 0;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (b < p.requests) prefix[b] = before + s - v;
+    carry += all;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[p.requests] = carry;
+  __syncthreads();
+}
+
+// Ranges of the line: worker w has tiles [w share, (w + 1) share).
+CEK_DEVICE int share_of(int total, int workers) { return max(1, (total + workers - 1) / workers); }
+
+// First tile of the line that worker's piece of a segment is kept under: slot
+// 2 w if it is the worker's first segment, 2 w + 1 if a later one.
+CEK_DEVICE int slot_of(int worker, int share, int seg_first) { return 2 * worker + (seg_first > worker * share ? 1 : 0); }
+
+CEK_DEVICE uint32_t movmatrix_t(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+CEK_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+CEK_DEVICE float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+CEK_DEVICE uint32_t lds_u32(uint32_t a) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
+  return r;
+}
+CEK_DEVICE uint2 lds_u64(uint32_t a) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
+  return r;
+}
+CEK_DEVICE uint32_t lds_u16(uint32_t a) {
+  uint16_t r;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(a));
+  return r;
+}
+CEK_DEVICE uint32_t lds_u8(uint32_t a) {
+  uint32_t r;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(a));
+  return r;
+}
+
+// The cursor that asks for pages: it runs STAGES tiles ahead of the arithmetic.
+// Page numbers come 32 at a time, one a lane, the next 32 asked for early.
+template <int D, int ROWS>
+struct Feeder {
+  using C = DecodeCfg<D>;
+  static constexpr int TK = C::TK;
+  const int32_t* row;      // the request's table row
+  const uint8_t* base;     // cache + head
+  int tile, left, end;     // tile of the request, tiles left in the segment
+  int window, ids, ids_next;
+
+  CEK_DEVICE void load(const AttnParams& p, const Segment& s, int skip, int lane) {
+    row = p.table + (int64_t)s.b * p.table_stride;
+    base = p.cache.data + (int64_t)s.h * p.cache.head_stride;
+    tile = s.r.tile0 + skip;
+    left = s.tiles - skip;
+    end = s.r.end;
+    window = tile * TK / p.P;
+    ids = page_id(p, window + lane);
+    ids_next = page_id(p, window + 32 + lane);
+  }
+  CEK_DEVICE int page_id(const AttnParams& p, int i) const {
+    return (int64_t)i * p.P < end ? min(max(__ldg(row + i), 0), p.cache.num_pages - 1) : 0;
+  }
+  // Asks for the tile into `dst`; the bytes complete on `bar`.
+  CEK_DEVICE void ask(const AttnParams& p, uint32_t dst, uint32_t bar, int lane) {
+    using L = Layout<D>;
+    const int key0 = tile * TK;
+    const int first = key0 / p.P;
+    if (first >= window + 32) {
+      window += 32;
+      ids = ids_next;
+      ids_next = page_id(p, window + 32 + lane);
+    }
+    if (p.P <= TK) {
+      const int pages = min(TK / p.P, max(0, (end - key0 + p.P - 1) / p.P));
+      const int id = __shfl_sync(0xffffffffu, ids, (first - window + lane) & 31);  // TK / P divides 32
+      const uint32_t bytes = (uint32_t)L::bytes(p.P);
+      if (lane == 0) mbar::arrive_expect_tx(bar, bytes * pages);
+      __syncwarp();
+      if (lane < pages) mbar::bulk_g2s(dst + lane * bytes, base + (int64_t)id * p.cache.page_stride, bytes, bar);
+    } else {
+      // part of a page: its four arrays, laid out as a page of TK tokens
+      const int id = __shfl_sync(0xffffffffu, ids, (first - window) & 31);
+      const int off = key0 % p.P;
+      const bool any = key0 < end;
+      if (lane == 0) mbar::arrive_expect_tx(bar, any ? (uint32_t)L::bytes(TK) : 0u);
+      __syncwarp();
+      if (any && lane < 4) {
+        const int width = (lane & 1) ? L::SCALE : L::CODE;
+        const int src = (lane >> 1) * L::v_code(p.P) + ((lane & 1) ? L::k_scale(p.P) : 0) + off * width;
+        const int to = (lane >> 1) * L::v_code(TK) + ((lane & 1) ? L::k_scale(TK) : 0);
+        mbar::bulk_g2s(dst + to, base + (int64_t)id * p.cache.page_stride + src, (uint32_t)(TK * width), bar);
+      }
+    }
+    ++tile;
+    --left;
+  }
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kDecodeThreads)
+attn_decode_kernel(const AttnParams p) {
+  using C = DecodeCfg<D>;
+  using L = Layout<D>;
+  constexpr int TK = C::TK, ROWS = 8 * NT, MT = TK / 16;
+  constexpr int WORDS = D / 32;       // 4-byte code words of a lane's share of a key
+  constexpr int STEPS = D / 16;       // k16 steps of the first product
+  constexpr int VW = D / 64;          // code words of a lane's channels of a value
+  constexpr int MI = 4 * VW;          // 16-channel row tiles of the second product
+  constexpr int VG = D == 256 ? 2 : 1;  // scale groups among a lane's value channels
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kDecodeWarps][C::STAGES];
+  __shared__ int32_t warp_sums[kDecodeWarps];
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem + kDecodeWarps * C::STAGES * C::STAGE);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+  pdl_launch_dependents();
+  if (lane == 0) {
+    for (int s = 0; s < C::STAGES; ++s) mbar::init(mbar::saddr(&bars[warp][s]), 1);
+    mbar::fence_init();
+  }
+  pdl_wait();
+  scan_requests<TK, ROWS>(p, prefix, warp_sums);
+  const int total = prefix[p.requests];
+  const int workers = (int)gridDim.x * kDecodeWarps;
+  const int worker = (int)blockIdx.x * kDecodeWarps + warp;
+  int share = share_of(total, workers);
+  int from = min(total, worker * share), to = min(total, from + share);
+  const uint32_t ring = mbar::saddr(smem) + warp * C::STAGES * C::STAGE;
+  const int BP = min(p.P, TK);              // tokens of a block in the ring
+  const int bp_shift = 31 - __clz(BP);
+
+  // ---- feed the ring
+  Feeder<D, ROWS> feed;
+  int asked = from;  // tile of the line that is asked for next
+  feed.left = 0;
+  auto ask = [&]() {
+    if (feed.left == 0) {
+      const Segment s = segment_at<TK, ROWS>(p, prefix, asked);
+      feed.load(p, s, asked - s.first, lane);
+    }
+    const int st = (asked - from) % C::STAGES;
+    feed.ask(p, ring + st * C::STAGE, mbar::saddr(&bars[warp][st]), lane);
+    ++asked;
+  };
+  for (int s = 0; s < C::STAGES && asked < to; ++s) ask();
+
+  bool dead = false;
+  int tile = from;
+  while (tile < to) {
+    // ---- a segment: its rows' queries as the first product's second operand
+    const Segment s = segment_at<TK, ROWS>(p, prefix, tile);
+    const int rows = s.r.n * p.group;
+    uint32_t qf[NT][STEPS][2];
+    float f[NT][2];          // score -> log2 units, per column
+    int hi[NT][2], lo[NT][2];  // visible keys of the column's row
+    int all_hi = INT32_MAX, all_lo = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = s.rb * ROWS + nt * 8 + g;
+      const int qi = r / p.group, tok = s.r.t0 + qi;
+      const bool real = r < rows && tok >= 0 && tok < p.tokens;
+      const T* src = static_cast<const T*>(p.q) + (int64_t)(real ? tok : 0) * p.qts +
+                     (int64_t)(s.h * p.group + (real ? r - qi * p.group : 0)) * p.qhs;
+      float unscale = 1.f;
+      uint4 v[WORDS];
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        const int d = D == 256 ? 32 * (t + 4 * (w >> 2)) + 8 * (w & 3) : t * (D / 4) + 8 * w;
+        v[w] = real ? *reinterpret_cast<const uint4*>(src + d) : make_uint4(0, 0, 0, 0);
+      }
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        uint32_t mx = 0;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w)
+          mx = __vmaxu2(__vmaxu2(__vmaxu2(v[w].x & 0x7FFF7FFFu, v[w].y & 0x7FFF7FFFu),
+                                 __vmaxu2(v[w].z & 0x7FFF7FFFu, v[w].w & 0x7FFF7FFFu)), mx);
+        mx = max(mx & 0xFFFFu, mx >> 16);
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const int e = (int)(mx >> 7);  // the largest channel is below 2^(e - 126)
+        // not finite: leave it; zero: nothing to scale
+        const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
+        const float up = __int_as_float((127 + k) << 23);
+        unscale = __int_as_float((127 - k) << 23);
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v[w]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 x = unpack2<T>(u[i]);
+            u[i] = pack2<__half>(x.x * up, x.y * up);
+          }
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        qf[nt][2 * w][0] = v[w].x;
+        qf[nt][2 * w][1] = v[w].y;
+        qf[nt][2 * w + 1][0] = v[w].z;
+        qf[nt][2 * w + 1][1] = v[w].w;
+      }
+      // this lane's columns are rows 2t, 2t + 1: their factors sit in lanes of those g
+      const float fr = p.scale_log2 * unscale * p.cache.scales[s.h];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f[nt][j] = __shfl_sync(0xffffffffu, fr, (2 * t + j) * 4);
+        const int c = s.rb * ROWS + nt * 8 + 2 * t + j;
+        const int pos = s.r.pos0 + c / p.group;
+        hi[nt][j] = c < rows ? min(pos + 1, s.r.end) : 0;
+        lo[nt][j] = p.window > 0 ? pos - p.window + 1 : 0;
+        if (c < rows) {
+          all_hi = min(all_hi, hi[nt][j]);
+          all_lo = max(all_lo, lo[nt][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, o));
+      all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, o));
+    }
+
+    float o[NT][MI][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
+    }
+    uint32_t nan_seen = 0;
+    const int piece0 = tile, stop = min(to, s.first + s.tiles);
+    for (; tile < stop; ++tile) {
+      const int st = (tile - from) % C::STAGES;
+      if (!dead && !mbar::wait(mbar::saddr(&bars[warp][st]), ((tile - from) / C::STAGES) & 1, kWaitPolls)) {
+        dead = true;
+        if (lane == 0) atomicAdd(&g_timeouts, 1ull);
+      }
+      dead = __any_sync(0xffffffffu, dead);
+      const uint32_t sb = ring + st * C::STAGE;
+      const int key0 = (s.r.tile0 + tile - s.first) * TK;
+      const bool whole = key0 + TK <= s.r.end;  // no slot of the tile is without a token
+
+      // ---- S^T = K Q^T
+      float sc[MT][NT][4];
+      const int kr = (g >> 1) + 4 * (g & 1);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int k16 = mt * 16;
+        const uint32_t blk = sb + (k16 >> bp_shift) * L::bytes(BP);
+        const int in = k16 & (BP - 1);
+        uint32_t w[2][WORDS], ks[2][WORDS / 2];
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+          const int key = in + kr + 8 * rr;
+          const uint32_t code = blk + key * L::CODE, sca = blk + L::k_scale(BP) + key * L::SCALE;
+          if constexpr (D == 64) {
+            const uint2 v = lds_u64(code + t * 8);
+            w[rr][0] = v.x;
+            w[rr][1] = v.y;
+            ks[rr][0] = lds_u8(sca + t);
+          } else {
+#pragma unroll
+            for (int j = 0; j < WORDS / 4; ++j) {
+              const uint4 v = mbar::lds16(code + (t + 4 * j) * 16);
+              w[rr][4 * j] = v.x;
+              w[rr][4 * j + 1] = v.y;
+              w[rr][4 * j + 2] = v.z;
+              w[rr][4 * j + 3] = v.w;
+              const uint32_t two = lds_u16(sca + (t + 4 * j) * 2);
+              ks[rr][2 * j] = two;
+              ks[rr][2 * j + 1] = two >> 8;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < WORDS / 2; ++j) {
+            const uint32_t b = ks[rr][j] & 0xFFu;
+            ks[rr][j] = fp8x2_to_f16x2<CEK_E4M3>(b | (b << 8));
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[mt][nt][j] = 0.f;
+#pragma unroll
+        for (int wd = 0; wd < WORDS; ++wd) {
+          uint32_t x[2][4];
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr) {
+            x[rr][0] = hmul2(e2m1x2_to_f16x2<0>(w[rr][wd]), ks[rr][wd / 2]);
+            x[rr][1] = hmul2(e2m1x2_to_f16x2<1>(w[rr][wd]), ks[rr][wd / 2]);
+            x[rr][2] = hmul2(e2m1x2_to_f16x2<2>(w[rr][wd]), ks[rr][wd / 2]);
+            x[rr][3] = hmul2(e2m1x2_to_f16x2<3>(w[rr][wd]), ks[rr][wd / 2]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(sc[mt][nt], x[0][0], x[1][0], x[0][1], x[1][1], qf[nt][2 * wd][0], qf[nt][2 * wd][1]);
+            mma16816(sc[mt][nt], x[0][2], x[1][2], x[0][3], x[1][3], qf[nt][2 * wd + 1][0], qf[nt][2 * wd + 1][1]);
+          }
+        }
+      }
+
+      // ---- softmax over the tile's keys (down the lanes of equal t)
+      const bool inside = key0 + TK <= all_hi && key0 >= all_lo;
+      float alpha[NT][2];
+      bool moved = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              float& v = sc[mt][nt][2 * rr + j];
+              v *= f[nt][j];
+              if (!inside) {
+                const int key = key0 + mt * 16 + rr * 8 + kr;
+                if (key >= hi[nt][j] || key < lo[nt][j]) v = -INFINITY;
+              }
+              top = fmaxf(top, v);
+            }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float now = fmaxf(m[nt][j], top);
+          const float base = (now == -INFINITY ? 0.f : now) - kShift;
+          alpha[nt][j] = now == m[nt][j] ? 1.f : ex2(m[nt][j] - now);
+          moved |= now != m[nt][j];
+          m[nt][j] = now;
+          float sum = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+              float& v = sc[mt][nt][2 * rr + j];
+              v = ex2(v - base);
+              sum += v;
+            }
+          l[nt][j] = l[nt][j] * alpha[nt][j] + sum;
+        }
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < MI; ++i) {
+            o[nt][i][0] *= alpha[nt][0];
+            o[nt][i][1] *= alpha[nt][1];
+            o[nt][i][2] *= alpha[nt][0];
+            o[nt][i][3] *= alpha[nt][1];
+          }
+      }
+
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t pf[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pf[nt][0] = movmatrix_t(pack2<__half>(sc[mt][nt][0], sc[mt][nt][1]));
+          pf[nt][1] = movmatrix_t(pack2<__half>(sc[mt][nt][2], sc[mt][nt][3]));
+        }
+        const int k16 = mt * 16;
+        const uint32_t blk = sb + (k16 >> bp_shift) * L::bytes(BP) + L::v_code(BP);
+        const int in = k16 & (BP - 1);
+        uint32_t w[4][VW], vs[2][VG];
+        uint32_t raw[VG];
+#pragma unroll
+        for (int j = 0; j < VG; ++j) raw[j] = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int key = in + t + 4 * q;
+          const uint32_t code = blk + key * L::CODE, sca = blk + BP * L::CODE + key * L::SCALE;
+          if constexpr (D == 64) {
+            w[q][0] = lds_u32(code + g * 4);
+            raw[0] |= lds_u8(sca + (g >> 1)) << (8 * q);
+          } else if constexpr (D == 128) {
+            const uint2 v = lds_u64(code + g * 8);
+            w[q][0] = v.x;
+            w[q][1] = v.y;
+            raw[0] |= lds_u8(sca + g) << (8 * q);
+          } else {
+            const uint4 v = mbar::lds16(code + g * 16);
+            w[q][0] = v.x;
+            w[q][1] = v.y;
+            w[q][2] = v.z;
+            w[q][3] = v.w;
+            const uint32_t two = lds_u16(sca + g * 2);
+            raw[0] |= (two & 0xFFu) << (8 * q);
+            raw[1] |= (two >> 8) << (8 * q);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < VG; ++j) {
+          if (!whole) {  // slots without a token: whatever they hold counts as zero
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (key0 + k16 + t + 4 * q >= s.r.end) raw[j] &= ~(0xFFu << (8 * q));
+          }
+          // a NaN scale must not reach rows that do not see its key (0 * NaN): it
+          // counts as zero here and is put in at the end of the segment
+          const uint32_t bad = ((raw[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+          nan_seen |= bad;
+          raw[j] &= ~((bad >> 7) * 0xFFu);
+          vs[0][j] = fp8x2_to_f16x2<CEK_E4M3, 0>(raw[j]);
+          vs[1][j] = fp8x2_to_f16x2<CEK_E4M3, 1>(raw[j]);
+        }
+#pragma unroll
+        for (int u = 0; u < VW; ++u) {
+          // byte i: channels 8u + 2i (even) and 8u + 2i + 1 (odd) of two keys
+          uint32_t even[2], odd[2];
+#pragma unroll
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const uint32_t a = w[2 * k2][u], b = w[2 * k2 + 1][u];
+            even[k2] = (a & 0x0F0F0F0Fu) | ((b << 4) & 0xF0F0F0F0u);
+            odd[k2] = ((a >> 4) & 0x0F0F0F0Fu) | (b & 0xF0F0F0F0u);
+          }
+          const uint32_t s0 = vs[0][VG == 2 ? u / 2 : 0], s1 = vs[1][VG == 2 ? u / 2 : 0];
+#define CEK_KV4_PV(I)                                                                                            \
+  {                                                                                                              \
+    const uint32_t a0 = hmul2(e2m1x2_to_f16x2<I>(even[0]), s0), a1 = hmul2(e2m1x2_to_f16x2<I>(odd[0]), s0);      \
+    const uint32_t a2 = hmul2(e2m1x2_to_f16x2<I>(even[1]), s1), a3 = hmul2(e2m1x2_to_f16x2<I>(odd[1]), s1);      \
+    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt)                                                            \
+      mma16816(o[nt][4 * u + I], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);                                          \
+  }
+          CEK_KV4_PV(0)
+          CEK_KV4_PV(1)
+          CEK_KV4_PV(2)
+          CEK_KV4_PV(3)
+#undef CEK_KV4_PV
+        }
+      }
+      __syncwarp();  // every lane has read the stage
+      if (asked < to && !dead) ask();
+    }
+
+    // ---- end of the segment, or of this worker's part of it
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 4);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 8);
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], 16);
+      }
+    if (__any_sync(0xffffffffu, nan_seen != 0)) {
+      // rare: look the keys' value scales up again, row by row
+      const int k0 = (s.r.tile0 + piece0 - s.first) * TK, k1 = min(s.r.end, (s.r.tile0 + stop - s.first) * TK);
+      for (int key = k0; key < k1; ++key) {
+        const int id = min(max(p.table[(int64_t)s.b * p.table_stride + key / p.P], 0), p.cache.num_pages - 1);
+        const uint8_t* sca = p.cache.data + (int64_t)id * p.cache.page_stride + (int64_t)s.h * p.cache.head_stride +
+                             L::v_scale(p.P) + (key % p.P) * L::SCALE;
+#pragma unroll
+        for (int gr = 0; gr < VG; ++gr) {
+          const bool nan = (sca[D == 64 ? g >> 1 : VG * g + gr] & 0x7F) == 0x7F;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (nan && key < hi[nt][j] && key >= lo[nt][j]) {
+#pragma unroll
+                for (int i = gr * (MI / VG); i < (gr + 1) * (MI / VG); ++i)
+                  o[nt][i][j] = o[nt][i][2 + j] = __int_as_float(0x7fffffff);
+              }
+        }
+      }
+    }
+    const bool mine = piece0 == s.first && stop == s.first + s.tiles;
+    const float vf = p.cache.scales[p.cache.heads + s.h];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int col = nt * 8 + 2 * t + j, c = s.rb * ROWS + col;
+        if (c >= rows) continue;
+        if (mine) {
+          const int qi = c / p.group, tok = s.r.t0 + qi;
+          if (tok < 0 || tok >= p.tokens) continue;
+          const float inv = l[nt][j] == 0.f ? 0.f : vf / l[nt][j];
+          T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(s.h * p.group + c - qi * p.group) * p.ohs +
+                   g * (D / 8);
+#pragma unroll
+          for (int i = 0; i < MI; i += 4)
+            *reinterpret_cast<uint4*>(dst + 2 * i) =
+                make_uint4(pack2<T>(o[nt][i][j] * inv, o[nt][i][2 + j] * inv),
+                           pack2<T>(o[nt][i + 1][j] * inv, o[nt][i + 1][2 + j] * inv),
+                           pack2<T>(o[nt][i + 2][j] * inv, o[nt][i + 2][2 + j] * inv),
+                           pack2<T>(o[nt][i + 3][j] * inv, o[nt][i + 3][2 + j] * inv));
+        } else {
+          float* slot = p.partial + (int64_t)slot_of(worker, share, s.first) * (ROWS * (D + 2));
+          if (g == 0) {
+            slot[col] = m[nt][j];
+            slot[ROWS + col] = l[nt][j];
+          }
+          float* dst = slot + 2 * ROWS + col * D + g * (D / 8);
+#pragma unroll
+          for (int i = 0; i < MI; i += 2)
+            *reinterpret_cast<float4*>(dst + 2 * i) =
+                make_float4(o[nt][i][j], o[nt][i][2 + j], o[nt][i + 1][j], o[nt][i + 1][2 + j]);
+        }
+      }
+  }
+  // a wait gave up: the copies that are still in flight land before the block ends (bounded)
+  if (dead)
+    for (int a = max(from, asked - C::STAGES); a < asked; ++a)
+      mbar::wait(mbar::saddr(&bars[warp][(a - from) % C::STAGES]), ((a - from) / C::STAGES) & 1, kWaitPolls);
+}
+
+// ---- joining the pieces of a segment --------------------------------------------
+// One warp per (request, kv head, row): weights 2^(m_i - m) over the pieces in
+// the order of the keys.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(128)
+attn_join_kernel(const AttnParams p, int workers) {
+  using C = DecodeCfg<D>;
+  constexpr int TK = C::TK, ROWS = 8 * NT, E = D / 32;
+  extern __shared__ __align__(16) int32_t prefix[];
+  __shared__ int32_t warp_sums[4];
+  pdl_launch_dependents();
+  pdl_wait();
+  scan_requests<TK, ROWS>(p, prefix, warp_sums);
+  const int b = blockIdx.y, lane = threadIdx.x & 31;
+  const Request r = request_of<TK>(p, b);
+  const int rows = r.n * p.group;
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 5);  // head x row
+  const int h = item / (p.max_q * p.group), c = item % (p.max_q * p.group);
+  if (h >= p.cache.heads || c >= rows) return;
+  const int rbs = (rows + ROWS - 1) / ROWS;
+  const int first = prefix[b] + (h * rbs + c / ROWS) * r.tiles, end = first + r.tiles;
+  const int share = share_of(prefix[p.requests], workers);
+  const int w0 = first / share, w1 = (end - 1) / share;
+  const int qi = c / p.group, tok = r.t0 + qi;
+  if (w0 == w1 || tok < 0 || tok >= p.tokens) return;  // one worker had it all
+  const int col = c % ROWS;
+  float top = -INFINITY;
+  for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, p.partial[(int64_t)slot_of(w, share, first) * (ROWS * (D + 2)) + col]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int w = w0; w <= w1; ++w) {
+    const float* slot = p.partial + (int64_t)slot_of(w, share, first) * (ROWS * (D + 2));
+    const float wt = ex2(slot[col] - base);
+    l += wt * slot[ROWS + col];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += wt * slot[2 * ROWS + col * D + lane * E + e];
+  }
+  const float inv = l == 0.f ? 0.f : p.cache.scales[p.cache.heads + h] / l;
+  T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(h * p.group + c - qi * p.group) * p.ohs + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(o[e] * inv);
+}
+
 }  // namespace kv4
 }  // namespace cek
+
+// ---- host side -------------------------------------------------------------------
+namespace {
+using namespace cek::kv4;
+
+struct DecodePlan {
+  int nt, ctas, workers;
+  size_t smem;
+  bool join;            // some segment may be in several pieces
+  int64_t partial_bytes;
+};
+
+template <int D>
+DecodePlan plan_decode_d(int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
+  using C = DecodeCfg<D>;
+  DecodePlan d;
+  const int64_t rows = max_q * group;
+  d.nt = rows <= 8 ? 1 : 2;
+  const int64_t per_request = heads * ((rows + 8 * d.nt - 1) / (8 * d.nt));
+  const int64_t tiles = std::max<int64_t>(1, (max_seq + C::TK - 1) / C::TK + 1);  // a window may start inside a tile
+  const int64_t req = std::min<int64_t>(requests, kMaxRequests);
+  d.smem = (size_t)kDecodeWarps * C::STAGES * C::STAGE + sizeof(int32_t) * (req + 1);
+  const int per_sm = 2 * (d.smem + 2048) <= 233472 ? 2 : 1;  // 228 KB of shared memory a SM
+  const int64_t most = (int64_t)per_sm * cek_host::sm_count();
+  const int64_t need = req * per_request >= most * kDecodeWarps ? most : (req * per_request * tiles + kDecodeWarps - 1) / kDecodeWarps;
+  d.ctas = (int)std::max<int64_t>(1, std::min(most, need));
+  d.workers = d.ctas * kDecodeWarps;
+  d.join = max_seq > C::TK;
+  d.partial_bytes = d.join ? 2ll * d.workers * 8 * d.nt * (D + 2) * (int64_t)sizeof(float) : 0;
+  return d;
+}
+DecodePlan plan_decode(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
+  return d == 64    ? plan_decode_d<64>(requests, heads, group, max_q, max_seq)
+         : d == 128 ? plan_decode_d<128>(requests, heads, group, max_q, max_seq)
+                    : plan_decode_d<256>(requests, heads, group, max_q, max_seq);
+}
+
+template <typename T, int D, int NT>
+int launch_decode(const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
+  static cek_host::DeviceSlots attr;
+  if (!cek_host::ensure_smem_attr(attr, attn_decode_kernel<T, D, NT>,
+                                  kDecodeWarps * DecodeCfg<D>::STAGES * DecodeCfg<D>::STAGE + 4 * (kMaxRequests + 1)))
+    return CEK_ERR_LAUNCH;
+  int s = cek_host::launch_pdl(attn_decode_kernel<T, D, NT>, dim3(d.ctas), dim3(kDecodeThreads), d.smem, st, p);
+  if (s != CEK_OK || !d.join) return s;
+  const dim3 grid((unsigned)(((int64_t)p.cache.heads * p.max_q * p.group + 3) / 4), (unsigned)p.requests);
+  return cek_host::launch_pdl(attn_join_kernel<T, D, NT>, grid, dim3(128), sizeof(int32_t) * (p.requests + 1), st, p, d.workers);
+}
+template <typename T>
+int launch_decode_t(int64_t dim, const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
+  if (dim == 64) return d.nt == 1 ? launch_decode<T, 64, 1>(p, d, st) : launch_decode<T, 64, 2>(p, d, st);
+  if (dim == 128) return d.nt == 1 ? launch_decode<T, 128, 1>(p, d, st) : launch_decode<T, 128, 2>(p, d, st);
+  return d.nt == 1 ? launch_decode<T, 256, 1>(p, d, st) : launch_decode<T, 256, 2>(p, d, st);
+}
+}  // namespace
 
 extern "C" int64_t cek_kv4_attention_workspace_bytes(int64_t requests, int64_t tokens, int64_t q_heads,
                                                      int64_t kv_heads, int64_t head_dim, int64_t max_query_len,
                                                      int64_t max_seq_len) {
-  return 0;
+  if (requests <= 0 || tokens <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || max_query_len <= 0 ||
+      max_seq_len <= 0 || !cek_host::kv4_head_dim(head_dim))
+    return 0;
+  return plan_decode(head_dim, requests, kv_heads, q_heads / kv_heads, std::min(max_query_len, tokens), max_seq_len).partial_bytes;
 }
 
 extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, const int32_t* block_table,
@@ -151,8 +903,25 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
   p.P = (int)cache->page_size;
   p.max_q = (int)std::min(max_query_len, tokens);
   p.max_seq = (int)max_seq_len;
+  p.key_limit = (int)(table_width * cache->page_size);
   p.window = (int)window;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  if (p.max_q * p.group <= 64) {
+    const DecodePlan d = plan_decode(cache->head_dim, requests, cache->kv_heads, p.group, p.max_q, max_seq_len);
+    if (workspace_bytes < d.partial_bytes || (d.partial_bytes > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
+    if (d.partial_bytes > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
+    p.partial = static_cast<float*>(workspace);
+    int rc = CEK_OK;
+    for (int64_t b = 0; b < requests && rc == CEK_OK; b += kMaxRequests) {  // the prefix sums of a launch are bounded
+      p.requests = (int)std::min<int64_t>(kMaxRequests, requests - b);
+      p.table = block_table + b * table_stride;
+      p.query_start = query_start + b;
+      p.seq_lens = seq_lens + b;
+      rc = dtype == CEK_F16 ? launch_decode_t<__half>(cache->head_dim, p, d, static_cast<cudaStream_t>(stream))
+                            : launch_decode_t<__nv_bfloat16>(cache->head_dim, p, d, static_cast<cudaStream_t>(stream));
+    }
+    return rc;
+  }
   const dim3 grid((unsigned)(((int64_t)p.max_q * q_heads + 3) / 4), (unsigned)requests), block(128);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto tag) {
