@@ -77,6 +77,7 @@ SIGNATURES = {
     "cek_kv4_gather": (_I, [_C, _P, _P, _P] + [_I64] * 5 + [_I, _P]),
     "cek_kv4_attention_workspace_bytes": (_I64, [_I64] * 7),
     "cek_kv4_attention": (_I, [_P, _C] + [_P] * 5 + [_I64] * 10 + [_F] + [_I64] * 3 + [_I, _P]),
+    "cek_kv4_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint64)]),
     "cek_gemv_fp8_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint64)]),
     "cek_gemm_fp8_timeouts": (_I, [ctypes.POINTER(ctypes.c_uint64)]),
 }

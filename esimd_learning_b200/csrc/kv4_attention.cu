@@ -1,7 +1,6 @@
 // kv4_attention.cu — attention over the paged 4-bit key/value cache
 // (cek_kv4_attention).
-#include "kv4.cuh"
-#include "mbarrier.cuh"
+#include "kv4_attention.cuh"
 
 #include <algorithm>
 #include <cmath>
@@ -9,100 +8,6 @@
 
 namespace cek {
 namespace kv4 {
-
-struct AttnParams {
-  const void* q;
-  void* out;
-  Cache cache;
-  const int32_t* table;
-  const int32_t* query_start;
-  const int32_t* seq_lens;
-  int64_t table_stride, qts, qhs, ots, ohs;
-  int requests, tokens, q_heads, group, table_width, P;
-  int max_q, max_seq, key_limit, window;  // key_limit: table_width * P
-  float scale_log2;  // softmax_scale * log2(e)
-  float* partial;    // pieces of split segments
-};
-
-// One warp per (token, query head): a lane scores one key of 32, then holds
-// D / 32 output channels of the weighted sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-attn_simple_kernel(const AttnParams p) {
-  using L = Layout<D>;
-  constexpr int E = D / 32;
-  __shared__ float qs[4][D];
-  pdl_launch_dependents();
-  pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 4 + warp;
-  const int req = blockIdx.y;
-  const int t0 = p.query_start[req], t1 = min(p.query_start[req + 1], p.tokens);
-  const int r = (int)(w / p.q_heads), h = (int)(w % p.q_heads);
-  const int n = p.query_start[req + 1] - t0;
-  if (r >= n || t0 + r >= t1 || t0 + r < 0) return;
-  const int seq = p.seq_lens[req];
-  const int pos = seq - n + r;
-  const int end = min(min(pos + 1, p.max_seq), p.table_width * p.P);
-  const int begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  const int kvh = h / p.group;
-  const T* q = static_cast<const T*>(p.q) + (int64_t)(t0 + r) * p.qts + h * p.qhs;
-  for (int i = lane; i < D; i += 32) qs[warp][i] = to_f32<T>(q[i]);
-  __syncwarp();
-  const float kf = p.cache.scales[kvh] * p.scale_log2, vf = p.cache.scales[p.cache.heads + kvh];
-  float m = -INFINITY, l = 0.f, o[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int k0 = begin; k0 < end; k0 += 32) {
-    const int key = k0 + lane;
-    float s = -INFINITY;
-    const uint8_t* block = p.cache.data;
-    int off = 0;
-    if (key < end) {
-      const int page = min(max(p.table[req * p.table_stride + key / p.P], 0), p.cache.num_pages - 1);
-      block += page * p.cache.page_stride + kvh * p.cache.head_stride;
-      off = key % p.P;
-      float acc = 0.f;
-      for (int gidx = 0; gidx < D / 16; ++gidx) {
-        const uint2 c = *reinterpret_cast<const uint2*>(block + off * L::CODE + gidx * 8);
-        const float sc = e4m3_to_f32(block[L::k_scale(p.P) + off * L::SCALE + gidx]);
-        float part = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const uint32_t code = ((j < 8 ? c.x : c.y) >> (4 * (j & 7))) & 15u;
-          part += unpack2<__half>(e2m1x2_to_f16x2<0>(code)).x * qs[warp][gidx * 16 + j];
-        }
-        acc += part * sc;
-      }
-      s = acc * kf;
-    }
-    const float top = fmaxf(m, warp_max(s));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float alpha = exp2f(m - base), pr = exp2f(s - base);
-    l = l * alpha + pr;
-    m = top;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= alpha;
-    const int cnt = min(32, end - k0);
-    for (int j = 0; j < cnt; ++j) {
-      const uint8_t* bj = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)block, j));
-      const int oj = __shfl_sync(0xffffffffu, off, j);
-      const float pj = __shfl_sync(0xffffffffu, pr, j);
-      const uint8_t* vc = bj + L::v_code(p.P) + oj * L::CODE;
-      const uint8_t* vs = bj + L::v_scale(p.P) + oj * L::SCALE;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int d = lane * E + e;
-        const uint32_t code = (vc[d >> 1] >> (4 * (d & 1))) & 15u;
-        o[e] += pj * (unpack2<__half>(e2m1x2_to_f16x2<0>(code)).x * e4m3_to_f32(vs[d >> 4]));
-      }
-    }
-  }
-  l = warp_sum(l);
-  T* out = static_cast<T*>(p.out) + (int64_t)(t0 + r) * p.ots + h * p.ohs;
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[lane * E + e] = from_f32<T>(l == 0.f ? 0.f : o[e] / l * vf);
-}
 
 // ---- decode ------------------------------------------------------------------
 // Few rows a request (single tokens, drafted tokens): the cache is read once
@@ -149,28 +54,6 @@ struct DecodeCfg {
   static constexpr int STAGE = Layout<D>::bytes(TK);
   static constexpr int STAGES = 3;
 };
-
-// What a request asks for, from its lengths.
-struct Request {
-  int t0, n;          // first token row, rows tokens (bounded)
-  int pos0;           // position of the first token
-  int tile0, tiles;   // tiles of TK keys that any row sees (at least one if n > 0: it writes the zeros)
-  int end;            // keys behind it do not exist
-};
-template <int TK>
-CEK_DEVICE Request request_of(const AttnParams& p, int b) {
-  Request r;
-  r.t0 = p.query_start[b];
-  const int n = max(p.query_start[b + 1] - r.t0, 0);
-  const int seq = p.seq_lens[b];
-  r.n = min(n, p.max_q);
-  r.pos0 = max(seq, 0) - n;  // a refused request (negative): every row stands before position 0
-  r.end = max(0, min(min(r.pos0 + r.n, p.max_seq), p.key_limit));
-  const int lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
-  r.tile0 = min(lo, r.end) / TK;
-  r.tiles = r.n > 0 ? max(1, (r.end + TK - 1) / TK - r.tile0) : 0;
-  return r;
-}
 
 struct Segment {
   int b, h, rb;
@@ -248,92 +131,6 @@ CEK_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-CEK_DEVICE float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-CEK_DEVICE uint32_t lds_u32(uint32_t a) {
-  uint32_t r;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(a));
-  return r;
-}
-CEK_DEVICE uint2 lds_u64(uint32_t a) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(a));
-  return r;
-}
-CEK_DEVICE uint32_t lds_u16(uint32_t a) {
-  uint16_t r;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(a));
-  return r;
-}
-CEK_DEVICE uint32_t lds_u8(uint32_t a) {
-  uint32_t r;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(r) : "r"(a));
-  return r;
-}
-
-// The cursor that asks for pages: it runs STAGES tiles ahead of the arithmetic.
-// Page numbers come 32 at a time, one a lane, the next 32 asked for early.
-template <int D, int ROWS>
-struct Feeder {
-  using C = DecodeCfg<D>;
-  static constexpr int TK = C::TK;
-  const int32_t* row;      // the request's table row
-  const uint8_t* base;     // cache + head
-  int tile, left, end;     // tile of the request, tiles left in the segment
-  int window, ids, ids_next;
-
-  CEK_DEVICE void load(const AttnParams& p, const Segment& s, int skip, int lane) {
-    row = p.table + (int64_t)s.b * p.table_stride;
-    base = p.cache.data + (int64_t)s.h * p.cache.head_stride;
-    tile = s.r.tile0 + skip;
-    left = s.tiles - skip;
-    end = s.r.end;
-    window = tile * TK / p.P;
-    ids = page_id(p, window + lane);
-    ids_next = page_id(p, window + 32 + lane);
-  }
-  CEK_DEVICE int page_id(const AttnParams& p, int i) const {
-    return (int64_t)i * p.P < end ? min(max(__ldg(row + i), 0), p.cache.num_pages - 1) : 0;
-  }
-  // Asks for the tile into `dst`; the bytes complete on `bar`.
-  CEK_DEVICE void ask(const AttnParams& p, uint32_t dst, uint32_t bar, int lane) {
-    using L = Layout<D>;
-    const int key0 = tile * TK;
-    const int first = key0 / p.P;
-    if (first >= window + 32) {
-      window += 32;
-      ids = ids_next;
-      ids_next = page_id(p, window + 32 + lane);
-    }
-    if (p.P <= TK) {
-      const int pages = min(TK / p.P, max(0, (end - key0 + p.P - 1) / p.P));
-      const int id = __shfl_sync(0xffffffffu, ids, (first - window + lane) & 31);  // TK / P divides 32
-      const uint32_t bytes = (uint32_t)L::bytes(p.P);
-      if (lane == 0) mbar::arrive_expect_tx(bar, bytes * pages);
-      __syncwarp();
-      if (lane < pages) mbar::bulk_g2s(dst + lane * bytes, base + (int64_t)id * p.cache.page_stride, bytes, bar);
-    } else {
-      // part of a page: its four arrays, laid out as a page of TK tokens
-      const int id = __shfl_sync(0xffffffffu, ids, (first - window) & 31);
-      const int off = key0 % p.P;
-      const bool any = key0 < end;
-      if (lane == 0) mbar::arrive_expect_tx(bar, any ? (uint32_t)L::bytes(TK) : 0u);
-      __syncwarp();
-      if (any && lane < 4) {
-        const int width = (lane & 1) ? L::SCALE : L::CODE;
-        const int src = (lane >> 1) * L::v_code(p.P) + ((lane & 1) ? L::k_scale(p.P) : 0) + off * width;
-        const int to = (lane >> 1) * L::v_code(TK) + ((lane & 1) ? L::k_scale(TK) : 0);
-        mbar::bulk_g2s(dst + to, base + (int64_t)id * p.cache.page_stride + src, (uint32_t)(TK * width), bar);
-      }
-    }
-    ++tile;
-    --left;
-  }
-};
-
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kDecodeThreads)
 attn_decode_kernel(const AttnParams p) {
@@ -368,13 +165,13 @@ attn_decode_kernel(const AttnParams p) {
   const int bp_shift = 31 - __clz(BP);
 
   // ---- feed the ring
-  Feeder<D, ROWS> feed;
+  Feeder<D, TK> feed;
   int asked = from;  // tile of the line that is asked for next
   feed.left = 0;
   auto ask = [&]() {
     if (feed.left == 0) {
       const Segment s = segment_at<TK, ROWS>(p, prefix, asked);
-      feed.load(p, s, asked - s.first, lane);
+      feed.load(p, s.b, s.h, s.r.tile0 + asked - s.first, s.first + s.tiles - asked, s.r.end, lane);
     }
     const int st = (asked - from) % C::STAGES;
     feed.ask(p, ring + st * C::STAGE, mbar::saddr(&bars[warp][st]), lane);
@@ -802,6 +599,8 @@ attn_join_kernel(const AttnParams p, int workers) {
 namespace {
 using namespace cek::kv4;
 
+constexpr int64_t kDecodeRows = 16;  // rows of a kv head that the decode kernel takes
+
 struct DecodePlan {
   int nt, ctas, workers;
   size_t smem;
@@ -859,7 +658,10 @@ extern "C" int64_t cek_kv4_attention_workspace_bytes(int64_t requests, int64_t t
   if (requests <= 0 || tokens <= 0 || kv_heads <= 0 || q_heads <= 0 || q_heads % kv_heads || max_query_len <= 0 ||
       max_seq_len <= 0 || !cek_host::kv4_head_dim(head_dim))
     return 0;
-  return plan_decode(head_dim, requests, kv_heads, q_heads / kv_heads, std::min(max_query_len, tokens), max_seq_len).partial_bytes;
+  const int64_t group = q_heads / kv_heads, max_q = std::min(max_query_len, tokens);
+  if (max_q * group <= kDecodeRows)
+    return plan_decode(head_dim, requests, kv_heads, group, max_q, max_seq_len).partial_bytes;
+  return cek::kv4::prefill_workspace(head_dim, requests, kv_heads, group, max_q, max_seq_len);
 }
 
 extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, const int32_t* block_table,
@@ -906,7 +708,7 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
   p.key_limit = (int)(table_width * cache->page_size);
   p.window = (int)window;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  if (p.max_q * p.group <= 64) {
+  if (p.max_q * p.group <= kDecodeRows) {
     const DecodePlan d = plan_decode(cache->head_dim, requests, cache->kv_heads, p.group, p.max_q, max_seq_len);
     if (workspace_bytes < d.partial_bytes || (d.partial_bytes > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
     if (d.partial_bytes > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
@@ -922,15 +724,18 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
     }
     return rc;
   }
-  const dim3 grid((unsigned)(((int64_t)p.max_q * q_heads + 3) / 4), (unsigned)requests), block(128);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto tag) {
-    using T = decltype(tag);
-    switch (cache->head_dim) {
-      case 64: return cek_host::launch_pdl(cek::kv4::attn_simple_kernel<T, 64>, grid, block, 0, st, p);
-      case 128: return cek_host::launch_pdl(cek::kv4::attn_simple_kernel<T, 128>, grid, block, 0, st, p);
-      default: return cek_host::launch_pdl(cek::kv4::attn_simple_kernel<T, 256>, grid, block, 0, st, p);
-    }
-  };
-  return dtype == CEK_F16 ? go(__half{}) : go(__nv_bfloat16{});
+  const int64_t need = cek::kv4::prefill_workspace(cache->head_dim, requests, cache->kv_heads, p.group, p.max_q, max_seq_len);
+  if (workspace_bytes < need || (need > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
+  if (need > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
+  p.partial = static_cast<float*>(workspace);
+  return cek::kv4::prefill_launch(dtype, cache->head_dim, p, max_seq_len, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int cek_kv4_timeouts(uint64_t* count) {
+  if (!count) return CEK_ERR_INVALID_ARG;
+  unsigned long long a = 0, b = 0;
+  if (cudaMemcpyFromSymbol(&a, cek::kv4::g_timeouts, sizeof(a)) != cudaSuccess || !cek::kv4::prefill_timeouts(&b))
+    return CEK_ERR_LAUNCH;
+  *count = a + b;
+  return CEK_OK;
 }

@@ -1,0 +1,599 @@
+// kv4_prefill.cu — attention over the paged 4-bit cache for many rows a
+// request (prompts, chunks): cek_kv4_attention's tcgen05 path.
+//
+// A CTA takes NQ x 128 rows (query token x head of the kv head's group) and the
+// tiles of TK keys that any of them sees.  16 warps:
+//  * softmax (one warpgroup per 128 rows, a thread a row): stages its row of Q
+//    in shared memory, then per tile reads S from tensor memory, keeps the
+//    running maximum and sum, and writes P (fp16) over S;
+//  * converters: turn the codes of a page into the fp16 operands, exactly
+//    (kv4.cuh), straight into the 128-byte-swizzled layout that the matrix unit
+//    reads; a four-slot ring K(j), V(j), K(j+1), ...
+//  * one warp copies pages (a bulk copy per page and half tile) into a raw ring;
+//  * one thread issues the matrix instructions: S = Q K^T with both operands in
+//    shared memory, O += P V with P in tensor memory and V read with keys as
+//    the strided dimension, so V needs no transpose.
+// With NQ = 2 the two row blocks take turns: while one's S is in softmax the
+// other's products run.  D = 256 fills tensor memory with one O, so NQ = 1 and
+// the tiles take turns instead (S double-buffered).
+//
+// Bounds at D = 128, per 256 rows x 128 keys: 2048 cycles of matrix unit, 2048
+// of exp2 (16 a cycle), ~2200 of shared memory (1536 of operand reads, 512 of
+// converted writes).
+//
+// The output is rescaled only when a row's maximum has grown by more than
+// 2^kLazy since the last time: P is at most 2^(kShift + kLazy) = 2^14 then,
+// inside fp16, and fp16 keeps P's full precision down to 2^-20 of the maximum.
+// Every wait is bounded; one that gives up is counted (cek_kv4_timeouts), the
+// CTA drains its copies and matrix instructions, frees its tensor memory and
+// returns.
+#include "kv4_attention.cuh"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace cek {
+namespace kv4 {
+
+__device__ unsigned long long g_timeouts_prefill;
+
+namespace pf {
+
+constexpr float kShift = 6.f, kLazy = 8.f;
+constexpr int kThreads = 512;
+constexpr uint32_t kPolls = 1u << 24;
+constexpr int kRaw = 3;  // raw stages: halves of a tile
+
+template <int D, int NQ>
+struct Cfg {
+  static constexpr int TK = D == 256 ? 64 : 128;
+  static constexpr int RK = TK / 2;                       // keys of a raw stage
+  static constexpr int ROWS = NQ * 128;
+  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2, RAW = Layout<D>::bytes(RK);
+  static constexpr int SMEM = Q_BYTES + 4 * SLOT + kRaw * RAW + 1024;
+  static constexpr int CONV_WARPS = NQ == 2 ? 4 : 8;      // warps 8..11, or 4..11
+  static constexpr int O_COL = 256;
+  static constexpr uint32_t IDESC_QK = (1u << 4) | (uint32_t(TK >> 3) << 17) | (8u << 24);
+  // bit 16: B (V) has its N dimension contiguous
+  static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (8u << 24);
+};
+
+CEK_DEVICE bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < kPolls; ++i) {
+    if (mbar::try_wait(bar, parity)) return true;
+    if ((i & 1023u) == 1023u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  atomicAdd(&g_timeouts_prefill, 1ull);
+  return false;
+}
+// The same by a whole warp, with one answer for all of it.
+CEK_DEVICE bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, wait(bar, parity, abort_flag));
+}
+CEK_DEVICE void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+CEK_DEVICE void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+CEK_DEVICE void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart;
+// `lead` is the distance of 64-element blocks where those are contiguous (V).
+CEK_DEVICE uint64_t desc(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+CEK_DEVICE void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+CEK_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+CEK_DEVICE void tmem_ld32(uint32_t addr, float* r) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+        "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+        "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr));
+}
+CEK_DEVICE void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+CEK_DEVICE void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+CEK_DEVICE void tmem_st16(uint32_t addr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
+      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]) : "memory");
+}
+CEK_DEVICE void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+CEK_DEVICE void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The rows and tiles of one CTA.
+struct Item {
+  int b, h, rb, split;
+  Request r;
+  int rows;            // of the request's kv head
+  int tile0, tiles;    // of this split
+  int limit;           // no row of the block sees a key at or past it
+};
+template <int TK, int ROWS>
+CEK_DEVICE bool item_of(const AttnParams& p, int row_blocks, int splits, Item& it) {
+  int64_t id = blockIdx.x;
+  it.split = (int)(id % splits);
+  id /= splits;
+  it.h = (int)(id % p.cache.heads);
+  id /= p.cache.heads;
+  it.b = (int)(id % p.requests);
+  it.rb = row_blocks - 1 - (int)(id / p.requests);  // the longest ranges first
+  it.r = request_of<TK>(p, it.b);
+  it.rows = it.r.n * p.group;
+  if (it.rb * ROWS >= it.rows) return false;
+  const int last = min(it.rows, (it.rb + 1) * ROWS) - 1;
+  const int lo = p.window > 0 ? max(0, it.r.pos0 + it.rb * ROWS / p.group - p.window + 1) : 0;
+  it.limit = min(it.r.pos0 + last / p.group + 1, it.r.end);
+  const int t0 = lo / TK, n = it.limit > lo ? (it.limit + TK - 1) / TK - t0 : 0;
+  const int a = (int)((int64_t)n * it.split / splits), z = (int)((int64_t)n * (it.split + 1) / splits);
+  it.tile0 = t0 + a;
+  it.tiles = z - a;
+  return true;
+}
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
+  using C = Cfg<D, NQ>;
+  using L = Layout<D>;
+  constexpr int TK = C::TK, RK = C::RK, ROWS = C::ROWS, GP = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t sbase = (mbar::saddr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t s_q = sbase, s_kv = sbase + C::Q_BYTES, s_rw = s_kv + 4 * C::SLOT;
+  __shared__ __align__(8) uint64_t raw_full[kRaw], raw_empty[kRaw], kv_full[4], kv_empty[4], s_full[2], p_full[2], o_done[2],
+      q_full, drain;
+  __shared__ uint32_t tmem_sh;
+  __shared__ volatile int abort_flag;
+  __shared__ volatile uint32_t nan_seen;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRaw; ++i) {
+      mbar::init(mbar::saddr(&raw_full[i]), 1);
+      mbar::init(mbar::saddr(&raw_empty[i]), C::CONV_WARPS);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar::init(mbar::saddr(&kv_full[i]), C::CONV_WARPS);
+      mbar::init(mbar::saddr(&kv_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar::init(mbar::saddr(&s_full[i]), 1);
+      mbar::init(mbar::saddr(&p_full[i]), 4);
+      mbar::init(mbar::saddr(&o_done[i]), 1);
+    }
+    mbar::init(mbar::saddr(&q_full), 4 * NQ);
+    mbar::init(mbar::saddr(&drain), 1);
+    abort_flag = 0;
+    nan_seen = 0;
+    mbar::fence_init();
+  }
+  pdl_wait();
+  Item it;
+  if (!item_of<TK, ROWS>(p, row_blocks, splits, it)) return;  // the whole block
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mbar::saddr(&tmem_sh)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tmem_sh;
+  const int n = it.tiles;
+  const bool soft = warp < 4 * NQ;
+
+  // what a softmax thread keeps until the end
+  const int x = NQ == 2 ? warp >> 2 : 0;                       // its stream of row blocks
+  const int rr = (warp & 3) * 32 + lane;                       // its row of the block
+  const int row = it.rb * ROWS + x * 128 + rr;
+  const int qi = row / p.group, tok = it.r.t0 + qi, head = it.h * p.group + row - qi * p.group;
+  const bool real = soft && row < it.rows && tok >= 0 && tok < p.tokens;
+  const int pos = it.r.pos0 + qi;
+  const int hi = row < it.rows ? min(pos + 1, it.r.end) : 0, lo = p.window > 0 ? pos - p.window + 1 : 0;
+  const uint32_t tm_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  float m = -INFINITY, l = 0.f, c = 0.f;
+
+  if (soft) {
+    if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // ---- Q: this thread's row, 16-byte chunk ch of 64-channel block cb at ch ^ (row & 7)
+    const T* src = static_cast<const T*>(p.q) + (int64_t)(real ? tok : 0) * p.qts + (int64_t)(real ? head : 0) * p.qhs;
+    const uint32_t dst = s_q + x * (128 * D * 2) + rr * 128;
+    float unscale = 1.f, up = 1.f;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      uint32_t mx = 0;
+      if (real) {
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 v = reinterpret_cast<const uint4*>(src)[i];
+          mx = __vmaxu2(__vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                                 __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)), mx);
+        }
+      }
+      mx = max(mx & 0xFFFFu, mx >> 16);
+      const int e = (int)(mx >> 7);  // as in the decode kernel: a power of two, exactly, into fp16's range
+      const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
+      up = __int_as_float((127 + k) << 23);
+      unscale = __int_as_float((127 - k) << 23);
+    }
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      uint4 v = real ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const float2 a = unpack2<T>(v.x), b = unpack2<T>(v.y), d = unpack2<T>(v.z), f = unpack2<T>(v.w);
+        v = make_uint4(pack2<__half>(a.x * up, a.y * up), pack2<__half>(b.x * up, b.y * up),
+                       pack2<__half>(d.x * up, d.y * up), pack2<__half>(f.x * up, f.y * up));
+      }
+      sts16(dst + (i >> 3) * (128 * 128) + (((i & 7) ^ (rr & 7)) << 4), v.x, v.y, v.z, v.w);
+    }
+    proxy_fence();
+    __syncwarp();
+    if (lane == 0) mbar::arrive(mbar::saddr(&q_full));
+    // score -> log2 units; not zero, so that a masked -inf stays -inf
+    c = fmaxf(p.scale_log2 * unscale * p.cache.scales[it.h], 1.2e-38f);
+    int whi = hi, wlo = lo;  // keys that every row of the warp sees
+    if (row >= it.rows) whi = INT32_MAX, wlo = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      whi = min(whi, __shfl_xor_sync(0xffffffffu, whi, o));
+      wlo = max(wlo, __shfl_xor_sync(0xffffffffu, wlo, o));
+    }
+    const uint32_t tm_o = tm_lane + C::O_COL + x * D;
+
+    for (int j = 0; j < n; ++j) {
+      const int buf = NQ == 2 ? x : j & 1;
+      const uint32_t par = NQ == 2 ? j & 1 : (j >> 1) & 1;
+      if (!wait_warp(mbar::saddr(&s_full[buf]), par, &abort_flag)) break;
+      fence_after();
+      const uint32_t tm_s = tm_lane + buf * 128;
+      float s[TK];
+#pragma unroll
+      for (int i = 0; i < TK; i += 32) tmem_ld32(tm_s + i, s + i);
+      tmem_ld_wait();
+      const int key0 = (it.tile0 + j) * TK;
+      if (key0 < wlo || key0 + TK > whi) {
+#pragma unroll
+        for (int i = 0; i < TK; ++i)
+          if (key0 + i < lo || key0 + i >= hi) s[i] = -INFINITY;
+      }
+      float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int i = 4; i < TK; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
+      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      const float now = fmaxf(m, mx);
+      // (a - b) * c of equal infinities is NaN: not a reason to rescale
+      const bool grow = (now - m) * c > kLazy;
+      if (__any_sync(0xffffffffu, grow)) {
+        if (j > 0) {
+          if (!wait_warp(mbar::saddr(&o_done[x]), (j - 1) & 1, &abort_flag)) break;
+          fence_after();
+          const float alpha = grow ? ex2((m - now) * c) : 1.f;
+          l *= alpha;
+#pragma unroll 1
+          for (int i = 0; i < D; i += 32) {
+            float o[32];
+            tmem_ld32(tm_o + i, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int q = 0; q < 32; ++q) o[q] *= alpha;
+            tmem_st16(tm_o + i, reinterpret_cast<uint32_t*>(o));
+            tmem_st16(tm_o + i + 16, reinterpret_cast<uint32_t*>(o) + 16);
+          }
+          tmem_st_wait();
+        }
+        if (grow) m = now;
+      }
+      const float bias = kShift - (m == -INFINITY ? 0.f : m * c);
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < TK; i += 32) {
+        uint32_t u[16];
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float a = ex2(__fmaf_rn(s[i + 2 * q], c, bias)), b = ex2(__fmaf_rn(s[i + 2 * q + 1], c, bias));
+          sum[0] += a;
+          sum[1] += b;
+          u[q] = pack2<__half>(a, b);
+        }
+        tmem_st16(tm_s + i / 2, u);
+      }
+      l += sum[0] + sum[1];
+      tmem_st_wait();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar::arrive(mbar::saddr(&p_full[buf]));
+    }
+    if (n > 0) wait(mbar::saddr(&o_done[x]), (n - 1) & 1, &abort_flag);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp < 12) {
+      // ---- converters: thread items are 16-channel groups of a key
+      const int ct = threadIdx.x - (12 - C::CONV_WARPS) * 32;
+      bool bad = false;
+      int raw = 0, slot = 0;  // stages and slots so far
+      for (int j = 0; j < n && !bad; ++j) {
+        for (int kv = 0; kv < 2 && !bad; ++kv, ++slot) {
+          if (!wait_warp(mbar::saddr(&kv_empty[slot & 3]), ((slot >> 2) & 1) ^ 1, &abort_flag)) { bad = true; break; }
+          const uint32_t out = s_kv + (slot & 3) * C::SLOT;
+          uint32_t nan = 0;
+          for (int half = 0; half < 2; ++half) {
+            const int rs = (raw + half) % kRaw;
+            if (kv == 0 && !wait_warp(mbar::saddr(&raw_full[rs]), ((raw + half) / kRaw) & 1, &abort_flag)) { bad = true; break; }
+            const uint32_t stage = s_rw + rs * C::RAW;
+            const int BP = min(p.P, RK), key0 = (it.tile0 + j) * TK + half * RK;
+#pragma unroll 4
+            for (int e = ct; e < RK * GP; e += C::CONV_WARPS * 32) {
+              const int key = e / GP, grp = e % GP;
+              const uint32_t blk = stage + (key / BP) * L::bytes(BP) + (kv ? L::v_code(BP) : 0);
+              const int in = key & (BP - 1);
+              const uint2 w = lds_u64(blk + in * L::CODE + grp * 8);
+              uint32_t sc = lds_u8(blk + BP * L::CODE + in * L::SCALE + grp);
+              if (kv) {
+                // slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
+                if (key0 + key >= it.limit) sc = 0;
+                if ((sc & 0x7F) == 0x7F) { nan = 1; sc = 0; }
+              }
+              const uint32_t s2 = fp8x2_to_f16x2<CEK_E4M3>(sc | (sc << 8));
+              const int r = half * RK + key;
+              const uint32_t dst = out + (grp >> 2) * (TK * 128) + r * 128;
+              const uint32_t ch = (grp & 3) * 2;
+              const uint32_t a0 = hmul2(e2m1x2_to_f16x2<0>(w.x), s2), a1 = hmul2(e2m1x2_to_f16x2<1>(w.x), s2),
+                             a2 = hmul2(e2m1x2_to_f16x2<2>(w.x), s2), a3 = hmul2(e2m1x2_to_f16x2<3>(w.x), s2);
+              const uint32_t b0 = hmul2(e2m1x2_to_f16x2<0>(w.y), s2), b1 = hmul2(e2m1x2_to_f16x2<1>(w.y), s2),
+                             b2 = hmul2(e2m1x2_to_f16x2<2>(w.y), s2), b3 = hmul2(e2m1x2_to_f16x2<3>(w.y), s2);
+              sts16(dst + ((ch ^ (r & 7)) << 4), a0, a1, a2, a3);
+              sts16(dst + (((ch + 1) ^ (r & 7)) << 4), b0, b1, b2, b3);
+            }
+            if (kv) {
+              __syncwarp();
+              if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));
+            }
+          }
+          if (bad) break;
+          if (nan) nan_seen = 1;
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0) mbar::arrive(mbar::saddr(&kv_full[slot & 3]));
+        }
+        raw += 2;
+      }
+    } else if (warp == 12) {
+      // ---- matrix instructions
+      if (lane == 0 && n > 0) {
+        bool ok = wait(mbar::saddr(&q_full), 0, &abort_flag);
+        auto qk = [&](int j, int st) {  // S = Q K^T into the stream's (tile's) buffer
+          const uint32_t d = tmem + (NQ == 2 ? st : j & 1) * 128;
+          const uint32_t a = s_q + st * (128 * D * 2), b = s_kv + ((2 * j) & 3) * C::SLOT;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            mma_ss(d, desc(a + (k >> 2) * (128 * 128) + (k & 3) * 32, 16), desc(b + (k >> 2) * (TK * 128) + (k & 3) * 32, 16),
+                   C::IDESC_QK, k > 0);
+          commit(mbar::saddr(&s_full[NQ == 2 ? st : j & 1]));
+        };
+        auto pv = [&](int j, int st) {  // O += P V
+          const uint32_t d = tmem + C::O_COL + st * D, a = tmem + (NQ == 2 ? st : j & 1) * 128;
+          const uint32_t b = s_kv + ((2 * j + 1) & 3) * C::SLOT;
+#pragma unroll
+          for (int k = 0; k < TK / 16; ++k)
+            mma_ts(d, a + k * 8, desc(b + k * 2048, TK * 128), C::IDESC_PV, j > 0 || k > 0);
+          commit(mbar::saddr(&o_done[st]));
+        };
+        auto kv_ready = [&](int i) { return wait(mbar::saddr(&kv_full[i & 3]), (i >> 2) & 1, &abort_flag); };
+        auto p_ready = [&](int j, int st) {
+          const bool r = wait(mbar::saddr(&p_full[NQ == 2 ? st : j & 1]), NQ == 2 ? j & 1 : (j >> 1) & 1, &abort_flag);
+          fence_after();
+          return r;
+        };
+        ok = ok && kv_ready(0);
+        if (ok) {
+          fence_after();
+          for (int st = 0; st < NQ; ++st) qk(0, st);
+          commit(mbar::saddr(&kv_empty[0]));
+        }
+        for (int j = 0; j < n && ok; ++j) {
+          if constexpr (NQ == 2) {
+            for (int st = 0; st < 2 && ok; ++st) {
+              ok = (st == 1 || kv_ready(2 * j + 1)) && p_ready(j, st);
+              if (!ok) break;
+              pv(j, st);
+              if (st == 1) commit(mbar::saddr(&kv_empty[(2 * j + 1) & 3]));
+              if (j + 1 < n) {
+                if (st == 0) ok = kv_ready(2 * j + 2);
+                if (!ok) break;
+                fence_after();
+                qk(j + 1, st);
+                if (st == 1) commit(mbar::saddr(&kv_empty[(2 * j + 2) & 3]));
+              }
+            }
+          } else {
+            if (j + 1 < n) {
+              ok = kv_ready(2 * j + 2);
+              if (!ok) break;
+              fence_after();
+              qk(j + 1, 0);
+              commit(mbar::saddr(&kv_empty[(2 * j + 2) & 3]));
+            }
+            ok = kv_ready(2 * j + 1) && p_ready(j, 0);
+            if (!ok) break;
+            pv(j, 0);
+            commit(mbar::saddr(&kv_empty[(2 * j + 1) & 3]));
+          }
+        }
+        commit(mbar::saddr(&drain));  // nothing of ours still runs when tensor memory is freed
+        wait(mbar::saddr(&drain), 0, &abort_flag);
+      }
+    } else if (warp == 13) {
+      // ---- pages
+      Feeder<D, RK> feed;
+      const int first = it.tile0 * 2, total = n * 2;
+      if (n > 0) feed.load(p, it.b, it.h, first, total, it.limit, lane);
+      int i = 0;
+      for (; i < total; ++i) {
+        if (!wait_warp(mbar::saddr(&raw_empty[i % kRaw]), ((i / kRaw) & 1) ^ 1, &abort_flag)) break;
+        feed.ask(p, s_rw + (i % kRaw) * C::RAW, mbar::saddr(&raw_full[i % kRaw]), lane);
+      }
+      for (int a = i > kRaw ? i - kRaw : 0; a < i; ++a)  // no copy of ours is still landing
+        wait(mbar::saddr(&raw_full[a % kRaw]), (a / kRaw) & 1, &abort_flag);
+    }
+  }
+
+  __syncthreads();
+  if (soft) {
+    // ---- the row's output
+    fence_after();
+    const float vf = p.cache.scales[p.cache.heads + it.h];
+    uint32_t nan_groups = 0;
+    if (nan_seen && real) {
+      // rare: which groups of 16 channels see a value that is NaN
+      const int k1 = min(hi, (it.tile0 + n) * TK);
+      for (int key = max(lo, it.tile0 * TK); key < k1; ++key) {
+        const int id = min(max(p.table[(int64_t)it.b * p.table_stride + key / p.P], 0), p.cache.num_pages - 1);
+        const uint8_t* sca = p.cache.data + (int64_t)id * p.cache.page_stride + (int64_t)it.h * p.cache.head_stride +
+                             L::v_scale(p.P) + (key % p.P) * L::SCALE;
+        for (int gr = 0; gr < GP; ++gr) nan_groups |= (uint32_t)((sca[gr] & 0x7F) == 0x7F) << gr;
+      }
+    }
+    const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : vf / l;
+    T* dst = static_cast<T*>(p.out) + (int64_t)(real ? tok : 0) * p.ots + (int64_t)(real ? head : 0) * p.ohs;
+    float* part = p.partial + (int64_t)blockIdx.x * (ROWS * (D + 2));
+    if (splits > 1) {
+      part[x * 128 + rr] = m == -INFINITY ? m : m * c;
+      part[ROWS + x * 128 + rr] = l;
+      part += 2 * ROWS + (x * 128 + rr) * D;
+    }
+#pragma unroll 1
+    for (int i = 0; i < D; i += 32) {
+      float o[32];
+      if (n > 0) {
+        tmem_ld32(tm_lane + C::O_COL + x * D + i, o);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int q = 0; q < 32; ++q) o[q] = 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < 32; ++q) {
+        o[q] *= inv;
+        if ((nan_groups >> ((i + q) >> 4)) & 1) o[q] = __int_as_float(0x7fffffff);
+      }
+      if (splits > 1) {
+#pragma unroll
+        for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(part + i + q) = make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]);
+      } else if (real) {
+#pragma unroll
+        for (int q = 0; q < 32; q += 8)
+          *reinterpret_cast<uint4*>(dst + i + q) = make_uint4(pack2<T>(o[q], o[q + 1]), pack2<T>(o[q + 2], o[q + 3]),
+                                                              pack2<T>(o[q + 4], o[q + 5]), pack2<T>(o[q + 6], o[q + 7]));
+      }
+    }
+    fence_before();
+  }
+  __syncthreads();
+  fence_after();
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+// Joins the splits of a row: one warp per row, D / 32 channels a lane.
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(128)
+attn_prefill_join_kernel(const AttnParams p, int row_blocks, int splits) {
+  using C = Cfg<D, NQ>;
+  constexpr int ROWS = C::ROWS, E = D / 32;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const Request r = request_of<C::TK>(p, b);
+  const int qi = row / p.group, tok = r.t0 + qi;
+  if (row >= r.n * p.group || tok < 0 || tok >= p.tokens) return;
+  const int rb = row / ROWS, col = row % ROWS;
+  const int64_t item = ((int64_t)(row_blocks - 1 - rb) * p.requests + b) * p.cache.heads + h;
+  const float* part = p.partial + item * splits * (ROWS * (D + 2));
+  float top = -INFINITY;
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, part[(int64_t)s * (ROWS * (D + 2)) + col]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float* q = part + (int64_t)s * (ROWS * (D + 2));
+    const float w = ex2(q[col] - base);
+    l += w * q[ROWS + col];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += w * q[2 * ROWS + col * D + lane * E + e];
+  }
+  const float inv = l == 0.f ? 0.f : p.cache.scales[p.cache.heads + h] / l;
+  T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(h * p.group + row - qi * p.group) * p.ohs + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(o[e] * inv);
+}
+
+struct Plan {
+  int nq, row_blocks, splits;
+  int64_t items, partial_bytes;
+};
+inline Plan plan_of(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
+  Plan r;
+  const int64_t rows = max_q * group;
+  r.nq = d == 256 || rows <= 128 ? 1 : 2;
+  r.row_blocks = (int)((rows + 128 * r.nq - 1) / (128 * r.nq));
+  r.items = requests * heads * r.row_blocks;
+  // too few row blocks for the SMs: split their keys, at least four tiles a piece
+  const int64_t tiles = (max_seq + (d == 256 ? 63 : 127)) / (d == 256 ? 64 : 128);
+  r.splits = 1;
+  if (r.items < cek_host::sm_count() && tiles >= 8)
+    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cek_host::sm_count() / r.items, tiles / 4));
+  r.partial_bytes = r.splits > 1 ? r.items * r.splits * 128 * r.nq * (d + 2) * (int64_t)sizeof(float) : 0;
+  return r;
+}
+
+template <typename T, int D, int NQ>
+int launch(const AttnParams& p, const Plan& r, cudaStream_t st) {
+  static cek_host::DeviceSlots attr;
+  if (!cek_host::ensure_smem_attr(attr, attn_prefill_kernel<T, D, NQ>, Cfg<D, NQ>::SMEM)) return CEK_ERR_LAUNCH;
+  const int64_t blocks = r.items * r.splits;
+  if (blocks > INT32_MAX) return CEK_ERR_INVALID_ARG;
+  int s = cek_host::launch_pdl(attn_prefill_kernel<T, D, NQ>, dim3((unsigned)blocks), dim3(kThreads), Cfg<D, NQ>::SMEM, st,
+                               p, r.row_blocks, r.splits);
+  if (s != CEK_OK || r.splits == 1) return s;
+  const dim3 grid((unsigned)(((int64_t)p.max_q * p.group + 3) / 4), (unsigned)p.cache.heads, (unsigned)p.requests);
+  return cek_host::launch_pdl(attn_prefill_join_kernel<T, D, NQ>, grid, dim3(128), 0, st, p, r.row_blocks, r.splits);
+}
+template <typename T>
+int launch_t(int64_t d, const AttnParams& p, const Plan& r, cudaStream_t st) {
+  if (d == 64) return r.nq == 1 ? launch<T, 64, 1>(p, r, st) : launch<T, 64, 2>(p, r, st);
+  if (d == 128) return r.nq == 1 ? launch<T, 128, 1>(p, r, st) : launch<T, 128, 2>(p, r, st);
+  return launch<T, 256, 1>(p, r, st);
+}
+}  // namespace pf
+
+int64_t prefill_workspace(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
+  return pf::plan_of(d, requests, heads, group, max_q, max_seq).partial_bytes;
+}
+int prefill_launch(int dtype, int64_t d, const AttnParams& p, int64_t max_seq, cudaStream_t st) {
+  const pf::Plan r = pf::plan_of(d, p.requests, p.cache.heads, p.group, p.max_q, max_seq);
+  return dtype == CEK_F16 ? pf::launch_t<__half>(d, p, r, st) : pf::launch_t<__nv_bfloat16>(d, p, r, st);
+}
+bool prefill_timeouts(unsigned long long* v) {
+  return cudaMemcpyFromSymbol(v, g_timeouts_prefill, sizeof(*v)) == cudaSuccess;
+}
+}  // namespace kv4
+}  // namespace cek
+

@@ -423,6 +423,9 @@ CEK_API int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, con
                               int64_t query_head_stride, int64_t out_token_stride,
                               int64_t out_head_stride, float softmax_scale, int64_t max_query_len,
                               int64_t max_seq_len, int64_t window, int dtype, void* stream);
+/* Bounded device waits in cek_kv4_attention's kernels that gave up since the
+ * library was loaded (0 in a healthy run).  Synchronous. */
+CEK_API int cek_kv4_timeouts(uint64_t* count);
 
 #ifdef __cplusplus
 }

@@ -578,3 +578,10 @@ def test_attention_wrong_tensors(ext, cuda_device):
             run_attention(ext, cuda_device, {**c, **bad}, out=torch.zeros_like(c["q"]) if "q" not in bad else None)
     with pytest.raises(RuntimeError):
         run_attention(ext, cuda_device, c, out=torch.zeros_like(c["q"])[:1])
+
+
+@pytest.mark.gpu
+def test_attention_no_wait_gave_up(cuda_device):
+    count = ctypes.c_uint64(1)
+    cabi.call("cek_kv4_timeouts", ctypes.byref(count))
+    assert count.value == 0
