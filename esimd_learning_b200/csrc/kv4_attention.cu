@@ -48,11 +48,15 @@ constexpr uint32_t kWaitPolls = 1u << 22;
 
 __device__ unsigned long long g_timeouts;
 
-template <int D>
+// Keys of a tile, CTAs of an SM (what the registers allow) and stages of a
+// warp's ring (what then fits into 228 KB).
+template <int D, int NT>
 struct DecodeCfg {
-  static constexpr int TK = D == 256 ? 32 : 64;                 // keys of a tile
+  static constexpr int TK = D == 256 ? 32 : 64;
   static constexpr int STAGE = Layout<D>::bytes(TK);
-  static constexpr int STAGES = 3;
+  static constexpr int PER_SM = D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? (NT == 1 ? 3 : 2) : 2;
+  static constexpr int STAGES = D == 64 ? (NT == 1 ? 3 : 4) : D == 128 ? (NT == 1 ? 2 : 3) : 3;
+  static constexpr int RING = kDecodeWarps * STAGES * STAGE;
 };
 
 struct Segment {
@@ -114,12 +118,31 @@ CEK_DEVICE void scan_requests(const AttnParams& p, int32_t* prefix, int32_t* war
   __syncthreads();
 }
 
-// Ranges of the line: worker w has tiles [w share, (w + 1) share).
-CEK_DEVICE int share_of(int total, int workers) { return max(1, (total + workers - 1) / workers); }
+// Ranges of the line: CTA c has tiles [c S, (c + 1) S), its warps four near-equal parts.
+struct Ranges {
+  int total, share;
+  CEK_DEVICE Ranges(int total_, int ctas) : total(total_), share(max(1, (total_ + ctas - 1) / ctas)) {}
+  CEK_DEVICE int at(int cta, int warp) const { return min(total, cta * share + share * warp / kDecodeWarps); }
+  CEK_DEVICE int cta_of(int tile) const { return tile / share; }
+  // The whole CTA is inside the segment: its warps' pieces become one.
+  CEK_DEVICE bool merged(int cta, int first, int end) const {
+    const int a = at(cta, 0), b = at(cta, kDecodeWarps);
+    return a < b && first <= a && b <= end;
+  }
+  // Where the piece of a segment is kept: a warp has a slot for its first
+  // segment and one for its last; a merged CTA uses its first warp's.
+  CEK_DEVICE int slot(int cta, int warp, int first, bool is_merged) const {
+    return is_merged ? 2 * kDecodeWarps * cta : 2 * (kDecodeWarps * cta + warp) + (first > at(cta, warp) ? 1 : 0);
+  }
+};
 
-// First tile of the line that worker's piece of a segment is kept under: slot
-// 2 w if it is the worker's first segment, 2 w + 1 if a later one.
-CEK_DEVICE int slot_of(int worker, int share, int seg_first) { return 2 * worker + (seg_first > worker * share ? 1 : 0); }
+// What the join has to know of a segment that starts in a warp's part and goes
+// beyond it (one a warp at most); rows = 0: none.  In front of the pieces.
+struct JoinItem {
+  int first, end, total;  // the segment's and all tiles
+  int t0, h, row0, rows;  // first token, kv head, the row block's first row, the kv head's rows
+  int pad;
+};
 
 CEK_DEVICE uint32_t movmatrix_t(uint32_t a) {
   uint32_t r;
@@ -132,9 +155,9 @@ CEK_DEVICE void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, u
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kDecodeThreads)
+__global__ void __launch_bounds__(kDecodeThreads, (DecodeCfg<D, NT>::PER_SM))
 attn_decode_kernel(const AttnParams p) {
-  using C = DecodeCfg<D>;
+  using C = DecodeCfg<D, NT>;
   using L = Layout<D>;
   constexpr int TK = C::TK, ROWS = 8 * NT, MT = TK / 16;
   constexpr int WORDS = D / 32;       // 4-byte code words of a lane's share of a key
@@ -145,7 +168,7 @@ attn_decode_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kDecodeWarps][C::STAGES];
   __shared__ int32_t warp_sums[kDecodeWarps];
-  int32_t* prefix = reinterpret_cast<int32_t*>(smem + kDecodeWarps * C::STAGES * C::STAGE);
+  int32_t* prefix = reinterpret_cast<int32_t*>(smem + C::RING);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
   pdl_launch_dependents();
@@ -155,14 +178,36 @@ attn_decode_kernel(const AttnParams p) {
   }
   pdl_wait();
   scan_requests<TK, ROWS>(p, prefix, warp_sums);
-  const int total = prefix[p.requests];
-  const int workers = (int)gridDim.x * kDecodeWarps;
-  const int worker = (int)blockIdx.x * kDecodeWarps + warp;
-  int share = share_of(total, workers);
-  int from = min(total, worker * share), to = min(total, from + share);
+  const Ranges ranges(prefix[p.requests], (int)gridDim.x);
+  const int from = ranges.at(blockIdx.x, warp), to = ranges.at(blockIdx.x, warp + 1);
+  bool merge = false;  // the CTA is inside one segment
+  if (ranges.at(blockIdx.x, 0) < ranges.total) {
+    const Segment s = segment_at<TK, ROWS>(p, prefix, ranges.at(blockIdx.x, 0));
+    merge = ranges.merged(blockIdx.x, s.first, s.first + s.tiles);
+  }
   const uint32_t ring = mbar::saddr(smem) + warp * C::STAGES * C::STAGE;
   const int BP = min(p.P, TK);              // tokens of a block in the ring
-  const int bp_shift = 31 - __clz(BP);
+  // where this lane's keys, values and scales of 16-key block mt start in a stage
+  const int kr = (g >> 1) + 4 * (g & 1);
+  uint32_t k_code[MT], k_sca[MT], v_code[MT], v_sca[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const uint32_t blk = (uint32_t)(mt * 16 / BP) * L::bytes(BP), in = (mt * 16) & (BP - 1);
+    k_code[mt] = blk + (in + kr) * L::CODE + t * (D == 64 ? 8 : 16);
+    k_sca[mt] = blk + L::k_scale(BP) + (in + kr) * L::SCALE + t * (D == 64 ? 1 : 2);
+    v_code[mt] = blk + L::v_code(BP) + (in + t) * L::CODE + g * (D / 16);
+    v_sca[mt] = blk + L::v_scale(BP) + (in + t) * L::SCALE + (D == 64 ? g >> 1 : VG * g);
+  }
+  // this lane's 16 bytes of the value scales, for the NaN check: their key and place
+  constexpr int KEYS16 = 16 / L::SCALE > 0 ? 16 / L::SCALE : 1;  // keys in 16 scale bytes
+  const int nan_key = lane * KEYS16;
+  const bool nan_lane = nan_key < TK;
+  const uint32_t nan_at = nan_lane ? (uint32_t)(nan_key / BP) * L::bytes(BP) + L::v_scale(BP) + (nan_key & (BP - 1)) * L::SCALE : 0;
+
+  JoinItem* items = reinterpret_cast<JoinItem*>(p.partial);
+  float* pieces = p.partial + (int64_t)gridDim.x * kDecodeWarps * (sizeof(JoinItem) / 4);
+  JoinItem* item = items + blockIdx.x * kDecodeWarps + warp;
+  if (p.partial && lane == 0) item->rows = 0;
 
   // ---- feed the ring
   Feeder<D, TK> feed;
@@ -235,7 +280,7 @@ attn_decode_kernel(const AttnParams p) {
         qf[nt][2 * w + 1][1] = v[w].w;
       }
       // this lane's columns are rows 2t, 2t + 1: their factors sit in lanes of those g
-      const float fr = p.scale_log2 * unscale * p.cache.scales[s.h];
+      const float fr = fmaxf(p.scale_log2 * unscale * p.cache.scales[s.h], 1.2e-38f);  // not 0: masked stays -inf
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         f[nt][j] = __shfl_sync(0xffffffffu, fr, (2 * t + j) * 4);
@@ -276,43 +321,32 @@ attn_decode_kernel(const AttnParams p) {
       dead = __any_sync(0xffffffffu, dead);
       const uint32_t sb = ring + st * C::STAGE;
       const int key0 = (s.r.tile0 + tile - s.first) * TK;
-      const bool whole = key0 + TK <= s.r.end;  // no slot of the tile is without a token
 
       // ---- S^T = K Q^T
       float sc[MT][NT][4];
-      const int kr = (g >> 1) + 4 * (g & 1);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int k16 = mt * 16;
-        const uint32_t blk = sb + (k16 >> bp_shift) * L::bytes(BP);
-        const int in = k16 & (BP - 1);
         uint32_t w[2][WORDS], ks[2][WORDS / 2];
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
-          const int key = in + kr + 8 * rr;
-          const uint32_t code = blk + key * L::CODE, sca = blk + L::k_scale(BP) + key * L::SCALE;
+          const uint32_t code = sb + k_code[mt] + 8 * rr * L::CODE, sca = sb + k_sca[mt] + 8 * rr * L::SCALE;
           if constexpr (D == 64) {
-            const uint2 v = lds_u64(code + t * 8);
+            const uint2 v = lds_u64(code);
             w[rr][0] = v.x;
             w[rr][1] = v.y;
-            ks[rr][0] = lds_u8(sca + t);
+            ks[rr][0] = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(lds_u8(sca)), 0, 0x1010);
           } else {
 #pragma unroll
             for (int j = 0; j < WORDS / 4; ++j) {
-              const uint4 v = mbar::lds16(code + (t + 4 * j) * 16);
+              const uint4 v = mbar::lds16(code + 64 * j);
               w[rr][4 * j] = v.x;
               w[rr][4 * j + 1] = v.y;
               w[rr][4 * j + 2] = v.z;
               w[rr][4 * j + 3] = v.w;
-              const uint32_t two = lds_u16(sca + (t + 4 * j) * 2);
-              ks[rr][2 * j] = two;
-              ks[rr][2 * j + 1] = two >> 8;
+              const uint32_t two = fp8x2_to_f16x2<CEK_E4M3>(lds_u16(sca + 8 * j));
+              ks[rr][2 * j] = __byte_perm(two, 0, 0x1010);
+              ks[rr][2 * j + 1] = __byte_perm(two, 0, 0x3232);
             }
-          }
-#pragma unroll
-          for (int j = 0; j < WORDS / 2; ++j) {
-            const uint32_t b = ks[rr][j] & 0xFFu;
-            ks[rr][j] = fp8x2_to_f16x2<CEK_E4M3>(b | (b << 8));
           }
         }
 #pragma unroll
@@ -345,25 +379,23 @@ attn_decode_kernel(const AttnParams p) {
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float top = -INFINITY;
+          if (!inside) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int rr = 0; rr < 2; ++rr) {
-              float& v = sc[mt][nt][2 * rr + j];
-              v *= f[nt][j];
-              if (!inside) {
+              for (int rr = 0; rr < 2; ++rr) {
                 const int key = key0 + mt * 16 + rr * 8 + kr;
-                if (key >= hi[nt][j] || key < lo[nt][j]) v = -INFINITY;
+                if (key >= hi[nt][j] || key < lo[nt][j]) sc[mt][nt][2 * rr + j] = -INFINITY;
               }
-              top = fmaxf(top, v);
-            }
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float now = fmaxf(m[nt][j], top);
-          const float base = (now == -INFINITY ? 0.f : now) - kShift;
-          alpha[nt][j] = now == m[nt][j] ? 1.f : ex2(m[nt][j] - now);
+          }
+          float now = m[nt][j];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) now = max3(now, sc[mt][nt][j], sc[mt][nt][2 + j]);
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 4));
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 8));
+          now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
+          const float bias = kShift - (now == -INFINITY ? 0.f : now * f[nt][j]);
+          alpha[nt][j] = now == m[nt][j] ? 1.f : ex2((m[nt][j] - now) * f[nt][j]);
           moved |= now != m[nt][j];
           m[nt][j] = now;
           float sum = 0.f;
@@ -372,7 +404,7 @@ attn_decode_kernel(const AttnParams p) {
 #pragma unroll
             for (int rr = 0; rr < 2; ++rr) {
               float& v = sc[mt][nt][2 * rr + j];
-              v = ex2(v - base);
+              v = ex2(__fmaf_rn(v, f[nt][j], bias));
               sum += v;
             }
           l[nt][j] = l[nt][j] * alpha[nt][j] + sum;
@@ -390,7 +422,19 @@ attn_decode_kernel(const AttnParams p) {
           }
       }
 
-      // ---- O^T += V^T P^T
+      // ---- O^T += V^T P^T.  A slot without a token or behind a row counts p = 0;
+      // a NaN scale must not turn that into NaN: it is 448 here, and the rows
+      // that see its key get their NaN at the end of the segment.
+      if (nan_lane && key0 + nan_key < s.r.end) {
+        uint4 v = mbar::lds16(sb + nan_at);
+        if (L::SCALE < 16 && key0 + nan_key + KEYS16 > s.r.end) {  // the last token is among the 16 bytes
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key0 + nan_key + 4 * i / L::SCALE >= s.r.end) u[i] = 0;
+        }
+        nan_seen |= nan_bytes(v);
+      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t pf[NT][2];
@@ -399,50 +443,36 @@ attn_decode_kernel(const AttnParams p) {
           pf[nt][0] = movmatrix_t(pack2<__half>(sc[mt][nt][0], sc[mt][nt][1]));
           pf[nt][1] = movmatrix_t(pack2<__half>(sc[mt][nt][2], sc[mt][nt][3]));
         }
-        const int k16 = mt * 16;
-        const uint32_t blk = sb + (k16 >> bp_shift) * L::bytes(BP) + L::v_code(BP);
-        const int in = k16 & (BP - 1);
         uint32_t w[4][VW], vs[2][VG];
         uint32_t raw[VG];
 #pragma unroll
         for (int j = 0; j < VG; ++j) raw[j] = 0;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int key = in + t + 4 * q;
-          const uint32_t code = blk + key * L::CODE, sca = blk + BP * L::CODE + key * L::SCALE;
+          const uint32_t code = sb + v_code[mt] + 4 * q * L::CODE, sca = sb + v_sca[mt] + 4 * q * L::SCALE;
           if constexpr (D == 64) {
-            w[q][0] = lds_u32(code + g * 4);
-            raw[0] |= lds_u8(sca + (g >> 1)) << (8 * q);
+            w[q][0] = lds_u32(code);
+            raw[0] |= lds_u8(sca) << (8 * q);
           } else if constexpr (D == 128) {
-            const uint2 v = lds_u64(code + g * 8);
+            const uint2 v = lds_u64(code);
             w[q][0] = v.x;
             w[q][1] = v.y;
-            raw[0] |= lds_u8(sca + g) << (8 * q);
+            raw[0] |= lds_u8(sca) << (8 * q);
           } else {
-            const uint4 v = mbar::lds16(code + g * 16);
+            const uint4 v = mbar::lds16(code);
             w[q][0] = v.x;
             w[q][1] = v.y;
             w[q][2] = v.z;
             w[q][3] = v.w;
-            const uint32_t two = lds_u16(sca + g * 2);
+            const uint32_t two = lds_u16(sca);
             raw[0] |= (two & 0xFFu) << (8 * q);
             raw[1] |= (two >> 8) << (8 * q);
           }
         }
 #pragma unroll
         for (int j = 0; j < VG; ++j) {
-          if (!whole) {  // slots without a token: whatever they hold counts as zero
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (key0 + k16 + t + 4 * q >= s.r.end) raw[j] &= ~(0xFFu << (8 * q));
-          }
-          // a NaN scale must not reach rows that do not see its key (0 * NaN): it
-          // counts as zero here and is put in at the end of the segment
-          const uint32_t bad = ((raw[j] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-          nan_seen |= bad;
-          raw[j] &= ~((bad >> 7) * 0xFFu);
-          vs[0][j] = fp8x2_to_f16x2<CEK_E4M3, 0>(raw[j]);
-          vs[1][j] = fp8x2_to_f16x2<CEK_E4M3, 1>(raw[j]);
+          vs[0][j] = scales_no_nan(raw[j]);
+          vs[1][j] = scales_no_nan(raw[j] >> 16);
         }
 #pragma unroll
         for (int u = 0; u < VW; ++u) {
@@ -504,8 +534,13 @@ attn_decode_kernel(const AttnParams p) {
         }
       }
     }
-    const bool mine = piece0 == s.first && stop == s.first + s.tiles;
+    const bool mine = !merge && piece0 == s.first && stop == s.first + s.tiles;
     const float vf = p.cache.scales[p.cache.heads + s.h];
+    if (p.partial && lane == 0 && piece0 == s.first && (merge ? s.first + s.tiles > ranges.at(blockIdx.x, kDecodeWarps) : !mine))
+      *item = {s.first, s.first + s.tiles, ranges.total, s.r.t0, s.h, s.rb * ROWS, rows, 0};
+    // the ring is free once this warp's only segment is done: a merged piece goes there
+    float* piece = merge ? reinterpret_cast<float*>(smem + warp * C::STAGES * C::STAGE)
+                         : pieces + (int64_t)ranges.slot(blockIdx.x, warp, s.first, false) * (ROWS * (D + 2));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -526,12 +561,11 @@ attn_decode_kernel(const AttnParams p) {
                            pack2<T>(o[nt][i + 2][j] * inv, o[nt][i + 2][2 + j] * inv),
                            pack2<T>(o[nt][i + 3][j] * inv, o[nt][i + 3][2 + j] * inv));
         } else {
-          float* slot = p.partial + (int64_t)slot_of(worker, share, s.first) * (ROWS * (D + 2));
           if (g == 0) {
-            slot[col] = m[nt][j];
-            slot[ROWS + col] = l[nt][j];
+            piece[col] = m[nt][j] == -INFINITY ? -INFINITY : m[nt][j] * f[nt][j];
+            piece[ROWS + col] = l[nt][j];
           }
-          float* dst = slot + 2 * ROWS + col * D + g * (D / 8);
+          float* dst = piece + 2 * ROWS + col * D + g * (D / 8);
 #pragma unroll
           for (int i = 0; i < MI; i += 2)
             *reinterpret_cast<float4*>(dst + 2 * i) =
@@ -543,53 +577,152 @@ attn_decode_kernel(const AttnParams p) {
   if (dead)
     for (int a = max(from, asked - C::STAGES); a < asked; ++a)
       mbar::wait(mbar::saddr(&bars[warp][(a - from) % C::STAGES]), ((a - from) / C::STAGES) & 1, kWaitPolls);
+  if (!merge) return;
+
+  // ---- the four warps' pieces of the one segment, in the order of the keys
+  const Segment s = segment_at<TK, ROWS>(p, prefix, ranges.at(blockIdx.x, 0));
+  const int rows = s.r.n * p.group;
+  const bool whole = ranges.at(blockIdx.x, 0) == s.first && ranges.at(blockIdx.x, kDecodeWarps) == s.first + s.tiles;
+  __syncthreads();
+  const float vf = p.cache.scales[p.cache.heads + s.h];
+  float* piece = pieces + (int64_t)ranges.slot(blockIdx.x, 0, s.first, true) * (ROWS * (D + 2));
+  for (int e = threadIdx.x; e < ROWS * (D / 8); e += kDecodeThreads) {
+    const int col = e / (D / 8), d = e % (D / 8) * 8, c = s.rb * ROWS + col;
+    if (c >= rows) continue;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w)
+      if (ranges.at(blockIdx.x, w) < ranges.at(blockIdx.x, w + 1))
+        top = fmaxf(top, reinterpret_cast<const float*>(smem + w * C::STAGES * C::STAGE)[col]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o[8] = {};
+#pragma unroll
+    for (int w = 0; w < kDecodeWarps; ++w) {
+      if (ranges.at(blockIdx.x, w) >= ranges.at(blockIdx.x, w + 1)) continue;
+      const float* q = reinterpret_cast<const float*>(smem + w * C::STAGES * C::STAGE);
+      const float wt = ex2(q[col] - base);
+      l += wt * q[ROWS + col];
+      const float4 x = *reinterpret_cast<const float4*>(q + 2 * ROWS + col * D + d);
+      const float4 y = *reinterpret_cast<const float4*>(q + 2 * ROWS + col * D + d + 4);
+      o[0] += wt * x.x; o[1] += wt * x.y; o[2] += wt * x.z; o[3] += wt * x.w;
+      o[4] += wt * y.x; o[5] += wt * y.y; o[6] += wt * y.z; o[7] += wt * y.w;
+    }
+    if (whole) {
+      const int qi = c / p.group, tok = s.r.t0 + qi;
+      if (tok < 0 || tok >= p.tokens) continue;
+      const float inv = l == 0.f ? 0.f : vf / l;
+      T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(s.h * p.group + c - qi * p.group) * p.ohs + d;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv),
+                                                  pack2<T>(o[4] * inv, o[5] * inv), pack2<T>(o[6] * inv, o[7] * inv));
+    } else {
+      if (d == 0) {
+        piece[col] = top;
+        piece[ROWS + col] = l;
+      }
+      float4* dst = reinterpret_cast<float4*>(piece + 2 * ROWS + col * D + d);
+      dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+    }
+  }
 }
 
 // ---- joining the pieces of a segment --------------------------------------------
-// One warp per (request, kv head, row): weights 2^(m_i - m) over the pieces in
-// the order of the keys.
+// CTA (c, y) joins the segments that decode CTA c's warps have left it, rows 2y
+// and 2y + 1 of the block: four warps a row, each every fourth piece, then the
+// four in order.
+constexpr int kJoinWarps = 4, kJoinRows = 2;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128)
-attn_join_kernel(const AttnParams p, int workers) {
-  using C = DecodeCfg<D>;
-  constexpr int TK = C::TK, ROWS = 8 * NT, E = D / 32;
-  extern __shared__ __align__(16) int32_t prefix[];
-  __shared__ int32_t warp_sums[4];
+__global__ void __launch_bounds__(32 * kJoinWarps * kJoinRows)
+attn_join_kernel(const AttnParams p, int ctas) {
+  constexpr int ROWS = 8 * NT, E = D / 32, SLOT = ROWS * (D + 2);
+  __shared__ JoinItem items[kDecodeWarps];
+  __shared__ float red[kJoinRows][kJoinWarps][D], red_l[kJoinRows][kJoinWarps];
   pdl_launch_dependents();
   pdl_wait();
-  scan_requests<TK, ROWS>(p, prefix, warp_sums);
-  const int b = blockIdx.y, lane = threadIdx.x & 31;
-  const Request r = request_of<TK>(p, b);
-  const int rows = r.n * p.group;
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 5);  // head x row
-  const int h = item / (p.max_q * p.group), c = item % (p.max_q * p.group);
-  if (h >= p.cache.heads || c >= rows) return;
-  const int rbs = (rows + ROWS - 1) / ROWS;
-  const int first = prefix[b] + (h * rbs + c / ROWS) * r.tiles, end = first + r.tiles;
-  const int share = share_of(prefix[p.requests], workers);
-  const int w0 = first / share, w1 = (end - 1) / share;
-  const int qi = c / p.group, tok = r.t0 + qi;
-  if (w0 == w1 || tok < 0 || tok >= p.tokens) return;  // one worker had it all
-  const int col = c % ROWS;
-  float top = -INFINITY;
-  for (int w = w0 + lane; w <= w1; w += 32) top = fmaxf(top, p.partial[(int64_t)slot_of(w, share, first) * (ROWS * (D + 2)) + col]);
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f, o[E];
+  const int cta = blockIdx.x, lane = threadIdx.x & 31, sub = (threadIdx.x >> 5) % kJoinWarps;
+  const int jr = (threadIdx.x >> 5) / kJoinWarps, col = blockIdx.y * kJoinRows + jr;
+  constexpr int WORDS = sizeof(JoinItem) / 4 * kDecodeWarps;
+  const float* pieces = p.partial + (int64_t)ctas * WORDS;
+  if (threadIdx.x < WORDS)
+    reinterpret_cast<int*>(items)[threadIdx.x] = reinterpret_cast<const int*>(p.partial)[cta * WORDS + threadIdx.x];
+  __syncthreads();
+  for (int w = 0; w < kDecodeWarps; ++w) {
+    const JoinItem s = items[w];
+    if (s.row0 + (int)blockIdx.y * kJoinRows >= s.rows) continue;
+    const Ranges ranges(s.total, ctas);
+    const int c = s.row0 + col, qi = c / p.group, tok = s.t0 + qi;
+    const bool real = c < s.rows && tok >= 0 && tok < p.tokens;
+    // pieces: warps of the first CTA, whole CTAs, warps of the last CTA
+    const int c1 = ranges.cta_of(s.end - 1);
+    const bool one0 = ranges.merged(cta, s.first, s.end), one1 = ranges.merged(c1, s.first, s.end);
+    const int n0 = one0 ? 1 : kDecodeWarps, mid = max(0, c1 - cta - 1);
+    const int count = n0 + mid + (c1 > cta ? (one1 ? 1 : kDecodeWarps) : 0);
+    auto slot_at = [&](int k) -> int {
+      if (k >= n0 && k < n0 + mid) return ranges.slot(cta + 1 + k - n0, 0, s.first, true);
+      const int kc = k < n0 ? cta : c1, kw = k < n0 ? k : k - n0 - mid;
+      if (k < n0 ? one0 : one1) return ranges.slot(kc, 0, s.first, true);
+      const int a = max(s.first, ranges.at(kc, kw)), b = min(s.end, ranges.at(kc, kw + 1));
+      return a < b ? ranges.slot(kc, kw, s.first, false) : -1;
+    };
+    float top = -INFINITY;
+    if (real)
+      for (int k = lane; k < count; k += 32) {
+        const int sl = slot_at(k);
+        if (sl >= 0) top = fmaxf(top, pieces[(int64_t)sl * SLOT + col]);
+      }
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
+    float l = 0.f, o[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int w = w0; w <= w1; ++w) {
-    const float* slot = p.partial + (int64_t)slot_of(w, share, first) * (ROWS * (D + 2));
-    const float wt = ex2(slot[col] - base);
-    l += wt * slot[ROWS + col];
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    if (real) {
+      for (int k0 = sub; k0 < count; k0 += 32 * kJoinWarps) {
+        // a piece a lane: its place and weight, then all of them in turn
+        const int mine = k0 + lane * kJoinWarps;
+        const int sl = mine < count ? slot_at(mine) : -1;
+        float wt = 0.f;
+        if (sl >= 0) {
+          wt = ex2(pieces[(int64_t)sl * SLOT + col] - base);
+          l += wt * pieces[(int64_t)sl * SLOT + ROWS + col];
+        }
+        const int n = min(32, (count - k0 + kJoinWarps - 1) / kJoinWarps);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+          const int si = __shfl_sync(0xffffffffu, sl, i);
+          const float wi = __shfl_sync(0xffffffffu, wt, i);
+          if (si < 0) continue;
+          const float* q = pieces + (int64_t)si * SLOT + 2 * ROWS + col * D + lane * E;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += wt * slot[2 * ROWS + col * D + lane * E + e];
+          for (int e = 0; e < E; ++e) o[e] += wi * q[e];
+        }
+      }
+    }
+    l = warp_sum(l);
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[jr][sub][lane * E + e] = o[e];
+    if (lane == 0) red_l[jr][sub] = l;
+    __syncthreads();
+    if (sub == 0 && real) {
+      l = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < kJoinWarps; ++i) {
+        l += red_l[jr][i];
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += red[jr][i][lane * E + e];
+      }
+      const float inv = l == 0.f ? 0.f : p.cache.scales[p.cache.heads + s.h] / l;
+      T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(s.h * p.group + c - qi * p.group) * p.ohs + lane * E;
+      uint32_t u[E / 2];
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) u[e] = pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+      if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = u[0];
+      else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
+      else *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    __syncthreads();
   }
-  const float inv = l == 0.f ? 0.f : p.cache.scales[p.cache.heads + h] / l;
-  T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(h * p.group + c - qi * p.group) * p.ohs + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(o[e] * inv);
 }
 
 }  // namespace kv4
@@ -602,30 +735,32 @@ using namespace cek::kv4;
 constexpr int64_t kDecodeRows = 16;  // rows of a kv head that the decode kernel takes
 
 struct DecodePlan {
-  int nt, ctas, workers;
+  int nt, ctas;
   size_t smem;
   bool join;            // some segment may be in several pieces
   int64_t partial_bytes;
 };
 
+template <int D, int NT>
+DecodePlan plan_decode_dn(int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
+  using C = DecodeCfg<D, NT>;
+  DecodePlan d;
+  d.nt = NT;
+  const int64_t req = std::min<int64_t>(requests, kMaxRequests);
+  const int64_t segments = req * heads * ((max_q * group + 8 * NT - 1) / (8 * NT));
+  const int64_t tiles = (max_seq + C::TK - 1) / C::TK + 1;  // a window may start inside a tile
+  d.smem = (size_t)C::RING + sizeof(int32_t) * (req + 1);
+  const int per_sm = (int)std::min<int64_t>(C::PER_SM, 233472 / (d.smem + 1024 + 512));  // 228 KB an SM, 1 KB a CTA reserved
+  const int64_t most = (int64_t)std::max(1, per_sm) * cek_host::sm_count();
+  d.ctas = (int)std::min(most, segments >= most ? most : segments * tiles);
+  d.join = max_seq > C::TK;
+  d.partial_bytes = d.join ? (int64_t)kDecodeWarps * d.ctas * (sizeof(JoinItem) + 2 * 8 * NT * (D + 2) * sizeof(float)) : 0;
+  return d;
+}
 template <int D>
 DecodePlan plan_decode_d(int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
-  using C = DecodeCfg<D>;
-  DecodePlan d;
-  const int64_t rows = max_q * group;
-  d.nt = rows <= 8 ? 1 : 2;
-  const int64_t per_request = heads * ((rows + 8 * d.nt - 1) / (8 * d.nt));
-  const int64_t tiles = std::max<int64_t>(1, (max_seq + C::TK - 1) / C::TK + 1);  // a window may start inside a tile
-  const int64_t req = std::min<int64_t>(requests, kMaxRequests);
-  d.smem = (size_t)kDecodeWarps * C::STAGES * C::STAGE + sizeof(int32_t) * (req + 1);
-  const int per_sm = 2 * (d.smem + 2048) <= 233472 ? 2 : 1;  // 228 KB of shared memory a SM
-  const int64_t most = (int64_t)per_sm * cek_host::sm_count();
-  const int64_t need = req * per_request >= most * kDecodeWarps ? most : (req * per_request * tiles + kDecodeWarps - 1) / kDecodeWarps;
-  d.ctas = (int)std::max<int64_t>(1, std::min(most, need));
-  d.workers = d.ctas * kDecodeWarps;
-  d.join = max_seq > C::TK;
-  d.partial_bytes = d.join ? 2ll * d.workers * 8 * d.nt * (D + 2) * (int64_t)sizeof(float) : 0;
-  return d;
+  return max_q * group <= 8 ? plan_decode_dn<D, 1>(requests, heads, group, max_q, max_seq)
+                            : plan_decode_dn<D, 2>(requests, heads, group, max_q, max_seq);
 }
 DecodePlan plan_decode(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
   return d == 64    ? plan_decode_d<64>(requests, heads, group, max_q, max_seq)
@@ -636,13 +771,12 @@ DecodePlan plan_decode(int64_t d, int64_t requests, int64_t heads, int64_t group
 template <typename T, int D, int NT>
 int launch_decode(const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
   static cek_host::DeviceSlots attr;
-  if (!cek_host::ensure_smem_attr(attr, attn_decode_kernel<T, D, NT>,
-                                  kDecodeWarps * DecodeCfg<D>::STAGES * DecodeCfg<D>::STAGE + 4 * (kMaxRequests + 1)))
+  if (!cek_host::ensure_smem_attr(attr, attn_decode_kernel<T, D, NT>, DecodeCfg<D, NT>::RING + 4 * (kMaxRequests + 1)))
     return CEK_ERR_LAUNCH;
   int s = cek_host::launch_pdl(attn_decode_kernel<T, D, NT>, dim3(d.ctas), dim3(kDecodeThreads), d.smem, st, p);
   if (s != CEK_OK || !d.join) return s;
-  const dim3 grid((unsigned)(((int64_t)p.cache.heads * p.max_q * p.group + 3) / 4), (unsigned)p.requests);
-  return cek_host::launch_pdl(attn_join_kernel<T, D, NT>, grid, dim3(128), sizeof(int32_t) * (p.requests + 1), st, p, d.workers);
+  return cek_host::launch_pdl(attn_join_kernel<T, D, NT>, dim3(d.ctas, 8 * NT / kJoinRows),
+                              dim3(32 * kJoinWarps * kJoinRows), 0, st, p, d.ctas);
 }
 template <typename T>
 int launch_decode_t(int64_t dim, const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
@@ -703,6 +837,7 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
   p.group = (int)(q_heads / cache->kv_heads);
   p.table_width = (int)table_width;
   p.P = (int)cache->page_size;
+  while ((1 << p.page_shift) < p.P) ++p.page_shift;
   p.max_q = (int)std::min(max_query_len, tokens);
   p.max_seq = (int)max_seq_len;
   p.key_limit = (int)(table_width * cache->page_size);
@@ -712,7 +847,7 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
     const DecodePlan d = plan_decode(cache->head_dim, requests, cache->kv_heads, p.group, p.max_q, max_seq_len);
     if (workspace_bytes < d.partial_bytes || (d.partial_bytes > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
     if (d.partial_bytes > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
-    p.partial = static_cast<float*>(workspace);
+    p.partial = d.join ? static_cast<float*>(workspace) : nullptr;
     int rc = CEK_OK;
     for (int64_t b = 0; b < requests && rc == CEK_OK; b += kMaxRequests) {  // the prefix sums of a launch are bounded
       p.requests = (int)std::min<int64_t>(kMaxRequests, requests - b);

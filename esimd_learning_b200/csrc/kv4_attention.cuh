@@ -15,7 +15,7 @@ struct AttnParams {
   const int32_t* query_start;
   const int32_t* seq_lens;
   int64_t table_stride, qts, qhs, ots, ohs;
-  int requests, tokens, q_heads, group, table_width, P;
+  int requests, tokens, q_heads, group, table_width, P, page_shift;  // P = 1 << page_shift
   int max_q, max_seq, key_limit, window;  // key_limit: table_width * P
   float scale_log2;  // softmax_scale * log2(e)
   float* partial;    // pieces of split segments
@@ -52,6 +52,39 @@ CEK_DEVICE float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+CEK_DEVICE uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+CEK_DEVICE void unpack_f32x2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+CEK_DEVICE uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+CEK_DEVICE uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+CEK_DEVICE float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// e4m3 scales of two keys or groups as f16x2; a NaN becomes 448, so that times
+// a probability of zero it is zero.
+CEK_DEVICE uint32_t scales_no_nan(uint32_t pair) {
+  uint32_t r;
+  asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(fp8x2_to_f16x2<CEK_E4M3>(pair)), "r"(0x5F005F00u));
+  return r;
+}
+// Whether any of 16 e4m3 bytes is NaN.
+CEK_DEVICE uint32_t nan_bytes(uint4 v) {
+  return (((v.x & 0x7F7F7F7Fu) + 0x01010101u) | ((v.y & 0x7F7F7F7Fu) + 0x01010101u) | ((v.z & 0x7F7F7F7Fu) + 0x01010101u) |
+          ((v.w & 0x7F7F7F7Fu) + 0x01010101u)) & 0x80808080u;
 }
 CEK_DEVICE uint32_t lds_u32(uint32_t a) {
   uint32_t r;
@@ -90,25 +123,25 @@ struct Feeder {
     tile = first;
     left = tiles;
     end = limit;
-    window = tile * TK / p.P;
+    window = (tile * TK) >> p.page_shift;
     ids = page_id(p, window + lane);
     ids_next = page_id(p, window + 32 + lane);
   }
   CEK_DEVICE int page_id(const AttnParams& p, int i) const {
-    return (int64_t)i * p.P < end ? min(max(__ldg(row + i), 0), p.cache.num_pages - 1) : 0;
+    return ((int64_t)i << p.page_shift) < end ? min(max(__ldg(row + i), 0), p.cache.num_pages - 1) : 0;
   }
   // Asks for the tile into `dst`; the bytes complete on `bar`.
   CEK_DEVICE void ask(const AttnParams& p, uint32_t dst, uint32_t bar, int lane) {
     using L = Layout<D>;
     const int key0 = tile * TK;
-    const int first = key0 / p.P;
+    const int first = key0 >> p.page_shift;
     if (first >= window + 32) {
       window += 32;
       ids = ids_next;
       ids_next = page_id(p, window + 32 + lane);
     }
     if (p.P <= TK) {
-      const int pages = min(TK / p.P, max(0, (end - key0 + p.P - 1) / p.P));
+      const int pages = min(TK >> p.page_shift, max(0, (end - key0 + p.P - 1) >> p.page_shift));
       const int id = __shfl_sync(0xffffffffu, ids, (first - window + lane) & 31);  // TK / P divides 32
       const uint32_t bytes = (uint32_t)L::bytes(p.P);
       if (lane == 0) mbar::arrive_expect_tx(bar, bytes * pages);
@@ -117,7 +150,7 @@ struct Feeder {
     } else {
       // part of a page: its four arrays, laid out as a page of TK tokens
       const int id = __shfl_sync(0xffffffffu, ids, (first - window) & 31);
-      const int off = key0 % p.P;
+      const int off = key0 & (p.P - 1);
       const bool any = key0 < end;
       if (lane == 0) mbar::arrive_expect_tx(bar, any ? (uint32_t)L::bytes(TK) : 0u);
       __syncwarp();

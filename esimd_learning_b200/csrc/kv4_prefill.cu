@@ -273,8 +273,12 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       }
       float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int i = 4; i < TK; ++i) top[i & 3] = fmaxf(top[i & 3], s[i]);
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      for (int i = 4; i < TK - 4; i += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top[q] = max3(top[q], s[i + 2 * q], s[i + 2 * q + 1]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) top[q] = fmaxf(top[q], s[TK - 4 + q]);
+      const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
       const float now = fmaxf(m, mx);
       // (a - b) * c of equal infinities is NaN: not a reason to rescale
       const bool grow = (now - m) * c > kLazy;
@@ -299,20 +303,25 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         if (grow) m = now;
       }
       const float bias = kShift - (m == -INFINITY ? 0.f : m * c);
-      float sum[2] = {0.f, 0.f};
+      const uint64_t c2 = f32x2(c, c), bias2 = f32x2(bias, bias);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < TK; i += 32) {
         uint32_t u[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          const float a = ex2(__fmaf_rn(s[i + 2 * q], c, bias)), b = ex2(__fmaf_rn(s[i + 2 * q + 1], c, bias));
-          sum[0] += a;
-          sum[1] += b;
+          float a, b;
+          unpack_f32x2(fma_f32x2(f32x2(s[i + 2 * q], s[i + 2 * q + 1]), c2, bias2), a, b);
+          a = ex2(a);
+          b = ex2(b);
+          sum[q & 1] = add_f32x2(sum[q & 1], f32x2(a, b));
           u[q] = pack2<__half>(a, b);
         }
         tmem_st16(tm_s + i / 2, u);
       }
-      l += sum[0] + sum[1];
+      float la, lb;
+      unpack_f32x2(add_f32x2(sum[0], sum[1]), la, lb);
+      l += la + lb;
       tmem_st_wait();
       fence_before();
       __syncwarp();
@@ -322,42 +331,61 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < 12) {
-      // ---- converters: thread items are 16-channel groups of a key
+      // ---- converters: thread items are 16-channel groups of a key, the same
+      // places in every half tile
+      constexpr int NTHR = C::CONV_WARPS * 32, ITEMS = RK * GP / NTHR;
       const int ct = threadIdx.x - (12 - C::CONV_WARPS) * 32;
+      const int BP = min(p.P, RK);
+      const uint32_t v_part = L::v_code(BP);
+      uint32_t from[ITEMS], from_s[ITEMS];
+#pragma unroll
+      for (int e = 0; e < ITEMS; ++e) {
+        const int key = (ct + e * NTHR) / GP, grp = (ct + e * NTHR) % GP, in = key & (BP - 1);
+        const uint32_t blk = (uint32_t)(key / BP) * L::bytes(BP);
+        from[e] = blk + in * L::CODE + grp * 8;
+        from_s[e] = blk + L::k_scale(BP) + in * L::SCALE + grp;
+      }
+      // item e's row is row0 + e NTHR / GP (a multiple of 8 apart, or the swizzle below would move)
+      static_assert((NTHR / GP) % 8 == 0, "rows of a thread's items differ by whole swizzle groups");
+      const int row0 = ct / GP, grp = ct % GP;
+      // the halves of 8 lanes write different 16-byte columns: groups 4.. write their second chunk first
+      const uint32_t flip = (grp >> 2) & 1;
+      const uint32_t at0 = (grp >> 2) * (TK * 128) + row0 * 128 + ((((grp & 3) * 2 + flip) ^ (row0 & 7)) << 4);
       bool bad = false;
       int raw = 0, slot = 0;  // stages and slots so far
       for (int j = 0; j < n && !bad; ++j) {
         for (int kv = 0; kv < 2 && !bad; ++kv, ++slot) {
           if (!wait_warp(mbar::saddr(&kv_empty[slot & 3]), ((slot >> 2) & 1) ^ 1, &abort_flag)) { bad = true; break; }
-          const uint32_t out = s_kv + (slot & 3) * C::SLOT;
-          uint32_t nan = 0;
+          const uint32_t out = s_kv + (slot & 3) * C::SLOT + at0;
           for (int half = 0; half < 2; ++half) {
             const int rs = (raw + half) % kRaw;
             if (kv == 0 && !wait_warp(mbar::saddr(&raw_full[rs]), ((raw + half) / kRaw) & 1, &abort_flag)) { bad = true; break; }
-            const uint32_t stage = s_rw + rs * C::RAW;
-            const int BP = min(p.P, RK), key0 = (it.tile0 + j) * TK + half * RK;
-#pragma unroll 4
-            for (int e = ct; e < RK * GP; e += C::CONV_WARPS * 32) {
-              const int key = e / GP, grp = e % GP;
-              const uint32_t blk = stage + (key / BP) * L::bytes(BP) + (kv ? L::v_code(BP) : 0);
-              const int in = key & (BP - 1);
-              const uint2 w = lds_u64(blk + in * L::CODE + grp * 8);
-              uint32_t sc = lds_u8(blk + BP * L::CODE + in * L::SCALE + grp);
-              if (kv) {
-                // slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
-                if (key0 + key >= it.limit) sc = 0;
-                if ((sc & 0x7F) == 0x7F) { nan = 1; sc = 0; }
+            const uint32_t stage = s_rw + rs * C::RAW + (kv ? v_part : 0);
+            const int key0 = (it.tile0 + j) * TK + half * RK + row0;
+            uint2 w[ITEMS];
+            uint32_t sc[ITEMS];
+#pragma unroll
+            for (int e = 0; e < ITEMS; ++e) {
+              w[e] = lds_u64(stage + from[e]);
+              sc[e] = lds_u8(stage + from_s[e]);
+            }
+            if (kv) {
+              // slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
+#pragma unroll
+              for (int e = 0; e < ITEMS; ++e) {
+                if (key0 + e * (NTHR / GP) >= it.limit) sc[e] = 0;
+                if ((sc[e] & 0x7F) == 0x7F) { nan_seen = 1; sc[e] = 0; }
               }
-              const uint32_t s2 = fp8x2_to_f16x2<CEK_E4M3>(sc | (sc << 8));
-              const int r = half * RK + key;
-              const uint32_t dst = out + (grp >> 2) * (TK * 128) + r * 128;
-              const uint32_t ch = (grp & 3) * 2;
-              const uint32_t a0 = hmul2(e2m1x2_to_f16x2<0>(w.x), s2), a1 = hmul2(e2m1x2_to_f16x2<1>(w.x), s2),
-                             a2 = hmul2(e2m1x2_to_f16x2<2>(w.x), s2), a3 = hmul2(e2m1x2_to_f16x2<3>(w.x), s2);
-              const uint32_t b0 = hmul2(e2m1x2_to_f16x2<0>(w.y), s2), b1 = hmul2(e2m1x2_to_f16x2<1>(w.y), s2),
-                             b2 = hmul2(e2m1x2_to_f16x2<2>(w.y), s2), b3 = hmul2(e2m1x2_to_f16x2<3>(w.y), s2);
-              sts16(dst + ((ch ^ (r & 7)) << 4), a0, a1, a2, a3);
-              sts16(dst + (((ch + 1) ^ (r & 7)) << 4), b0, b1, b2, b3);
+            }
+#pragma unroll
+            for (int e = 0; e < ITEMS; ++e) {
+              const uint32_t s2 = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(sc[e]), 0, 0x1010);
+              const uint32_t x = flip ? w[e].y : w[e].x, y = flip ? w[e].x : w[e].y;
+              const uint32_t dst = out + (half * RK + e * (NTHR / GP)) * 128;
+              sts16(dst, hmul2(e2m1x2_to_f16x2<0>(x), s2), hmul2(e2m1x2_to_f16x2<1>(x), s2),
+                    hmul2(e2m1x2_to_f16x2<2>(x), s2), hmul2(e2m1x2_to_f16x2<3>(x), s2));
+              sts16(dst ^ 16, hmul2(e2m1x2_to_f16x2<0>(y), s2), hmul2(e2m1x2_to_f16x2<1>(y), s2),
+                    hmul2(e2m1x2_to_f16x2<2>(y), s2), hmul2(e2m1x2_to_f16x2<3>(y), s2));
             }
             if (kv) {
               __syncwarp();
@@ -365,7 +393,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
             }
           }
           if (bad) break;
-          if (nan) nan_seen = 1;
           proxy_fence();
           __syncwarp();
           if (lane == 0) mbar::arrive(mbar::saddr(&kv_full[slot & 3]));
