@@ -5,154 +5,241 @@
 #include "kv4.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace cek {
 namespace kv4 {
 
-// ---- append ------------------------------------------------------------------
-// One thread per 16-channel group of one token and head, keys and values in one
-// grid.  The D/16 threads of a head lie side by side in a warp: their code
-// bytes are one contiguous store, their scale bytes are gathered into one.
+// ---- append and gather -------------------------------------------------------
+// Both move 16-bit values on one side and 4.5 bits a value on the other: HBM is
+// their bound, and the instructions around 16 bytes are what competes with it.
+// A gather thread takes 8 channels, 16 bytes of the 16-bit side, of both the key
+// and the value of a unit (token, head): D/8 neighbouring lanes have a unit,
+// every access of a warp is contiguous, and a unit's place is worked out once.
+// An append thread takes a whole group of 16, so that the scale is worked out
+// once.  Long calls give a thread U = 2 units, their loads in flight together;
+// short ones one, for more threads.
 template <typename T, bool VEC>
-CEK_DEVICE void load_group(const T* p, float (&x)[16]) {
+CEK_DEVICE uint4 load8(const T* p) {
+  if constexpr (VEC) return ldg_nc(p);
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = e[2 * i] | ((uint32_t)e[2 * i + 1] << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T, bool VEC>
+CEK_DEVICE void store8(T* p, uint4 v) {
   if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(p) = v;
+  } else {
+    uint16_t* e = reinterpret_cast<uint16_t*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 v = ldg_nc(p + 8 * h);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int i = 0; i < 4; ++i) {
+      e[2 * i] = (uint16_t)w[i];
+      e[2 * i + 1] = (uint16_t)(w[i] >> 16);
+    }
+  }
+}
+
+// Division of n < 2^31 by a number that the launch fixes, as a multiplication:
+// n / d = (mulhi(n, m) + n) >> s with s = ceil(log2 d), m = floor(2^32 (2^s - d) / d) + 1.
+struct Divisor {
+  uint32_t d, m, s;
+  explicit Divisor(uint32_t d_) : d(d_), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)((((1ull << s) - d) << 32) / d) + 1;
+  }
+};
+CEK_DEVICE uint32_t divide(uint32_t n, const Divisor& d) { return (__umulhi(n, d.m) + n) >> d.s; }
+// Unit number -> token, head.
+CEK_DEVICE int2 token_head(uint32_t u, const Divisor& n) {
+  const uint32_t t = divide(u, n);
+  return make_int2((int)t, (int)(u - t * n.d));
+}
+
+// Codes and scale byte of a group of 16 channels.
+template <typename T>
+CEK_DEVICE uint2 quantize16(const uint4 (&v)[2], float g, uint32_t& s8) {
+  const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+  // largest magnitude: 16-bit patterns without their sign order as their values, a NaN above infinity
+  uint32_t mx = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<T>(w[i]);
-        x[8 * h + 2 * i] = f.x;
-        x[8 * h + 2 * i + 1] = f.y;
-      }
+  for (int j = 0; j < 8; ++j) mx = __vmaxu2(mx, w[j] & 0x7FFF7FFFu);
+  const float a = unpack2<T>(max(mx & 0xFFFFu, mx >> 16)).x;
+  s8 = __nv_cvt_float_to_fp8(__fdiv_rn(a, __fmul_rn(6.f, g)), __NV_SATFINITE, __NV_E4M3);
+  const float unit = __fmul_rn(e4m3_to_f32(s8), g);
+  uint32_t code[2] = {0, 0};
+  if (unit > 0x1p-60f && unit < 0x1p60f && a < 0x1p100f) {
+    // x / unit correctly rounded without a division per channel, as in
+    // quant_fp8_per_token_kernel (Markstein: the correctly rounded reciprocal and
+    // two corrections), two channels an instruction.  On -x, so that the
+    // remainder q unit - x of a zero is +0 and the quotient keeps its sign.
+    const float y = __frcp_rn(unit);
+    const uint64_t n2 = f32x2(-y, -y), u2 = f32x2(unit, unit);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 x = unpack2<T>(w[j] ^ 0x80008000u);
+      const uint64_t x2 = f32x2(x.x, x.y);
+      uint64_t q = mul_f32x2(x2, n2);
+      q = fma_f32x2(fma_f32x2(q, u2, x2), n2, q);
+      q = fma_f32x2(fma_f32x2(q, u2, x2), n2, q);
+      float2 r;
+      unpack_f32x2(q, r.x, r.y);
+      code[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp4x2(r, __NV_E2M1, cudaRoundNearest) << (8 * (j & 3));
     }
   } else {
+    // a unit far from 1 (or zero, or NaN)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = to_f32<T>(p[i]);
+    for (int j = 0; j < 8; ++j) {
+      const float2 x = unpack2<T>(w[j]);
+      const float2 r = make_float2(unit == 0.f ? 0.f : __fdiv_rn(x.x, unit), unit == 0.f ? 0.f : __fdiv_rn(x.y, unit));
+      code[j >> 2] |= (uint32_t)__nv_cvt_float2_to_fp4x2(r, __NV_E2M1, cudaRoundNearest) << (8 * (j & 3));
+    }
   }
+  return make_uint2(code[0], code[1]);
 }
 
-template <typename T, int D, bool VEC>
+template <typename T, int D, bool VEC, int U>
 __global__ void __launch_bounds__(256)
 append_kernel(const T* __restrict__ key, const T* __restrict__ value, const int64_t* __restrict__ slots, Cache c,
-              int P, int64_t groups, int64_t kts, int64_t khs, int64_t vts, int64_t vhs) {
+              int shift, uint32_t units, const Divisor heads, int64_t kts, int64_t khs, int64_t vts, int64_t vhs) {
   using L = Layout<D>;
-  constexpr int GP = D / 16;
+  constexpr int LANES = D / 16, PER = 256 / LANES;
+  const int P = 1 << shift;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const bool live = id < groups;
-  const int64_t u = live ? id : groups - 1;
-  const int grp = (int)(u % GP);
-  const int64_t head_row = u / GP;                 // (token, k or v, head)
-  const int h = (int)(head_row % c.heads);
-  const int64_t r = head_row / c.heads;
-  const int kv = (int)(r & 1);
-  const int64_t t = r >> 1;
-  const int64_t slot = slots[t];
-  const bool store = live && slot >= 0 && slot < (int64_t)c.num_pages * P;
-  const T* src = kv ? value + t * vts + h * vhs : key + t * kts + h * khs;
-  float x[16];
-  load_group<T, VEC>(src + grp * 16, x);
-  float a = 0.f;
-  bool nan = false;
+  const int ln = threadIdx.x % LANES;  // its group of 16 channels
+  const uint32_t u0 = blockIdx.x * (PER * U) + threadIdx.x / LANES;
+  uint4 x[U][2][2];  // [unit][k, v][halves]
+  int64_t slot[U];
+  int h[U];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    a = fmaxf(a, fabsf(x[i]));  // fmaxf drops a NaN: remembered beside it
-    nan |= x[i] != x[i];
+  for (int i = 0; i < U; ++i) {
+    const uint32_t u = u0 + i * PER;
+    const int2 n = token_head(min(u, units - 1), heads);
+    h[i] = n.y;
+    slot[i] = u < units ? slots[n.x] : -1;
+    const T* k = key + (int64_t)n.x * kts + n.y * khs + ln * 16;
+    const T* v = value + (int64_t)n.x * vts + n.y * vhs + ln * 16;
+    x[i][0][0] = load8<T, VEC>(k);
+    x[i][0][1] = load8<T, VEC>(k + 8);
+    x[i][1][0] = load8<T, VEC>(v);
+    x[i][1][1] = load8<T, VEC>(v + 8);
   }
-  if (nan) a = __int_as_float(0x7fffffff);
-  const float g = c.scales[kv * c.heads + h];
-  const uint32_t s8 = __nv_cvt_float_to_fp8(__fdiv_rn(a, __fmul_rn(6.f, g)), __NV_SATFINITE, __NV_E4M3);
-  const float unit = __fmul_rn(e4m3_to_f32(s8), g);
-  uint32_t w[2] = {0u, 0u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 y = make_float2(unit == 0.f ? 0.f : __fdiv_rn(x[2 * i], unit),
-                                 unit == 0.f ? 0.f : __fdiv_rn(x[2 * i + 1], unit));
-    w[i >> 2] |= (uint32_t)__nv_cvt_float2_to_fp4x2(y, __NV_E2M1, cudaRoundNearest) << (8 * (i & 3));
+  for (int i = 0; i < U; ++i) {
+    const bool store = slot[i] >= 0 && slot[i] < (int64_t)c.num_pages << shift;
+    uint8_t* block = c.data + (store ? (slot[i] >> shift) * c.page_stride + (int64_t)h[i] * c.head_stride : 0);
+    const int off = (int)slot[i] & (P - 1);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      uint32_t s8;
+      const uint2 code = quantize16<T>(x[i][kv], c.scales[kv * c.heads + h[i]], s8);
+      // the scales of four groups as one word
+      s8 <<= 8 * (ln & 3);
+      s8 |= __shfl_xor_sync(0xffffffffu, s8, 1);
+      s8 |= __shfl_xor_sync(0xffffffffu, s8, 2);
+      if (!store) continue;
+      uint8_t* part = block + (kv ? L::v_code(P) : 0);
+      *reinterpret_cast<uint2*>(part + off * L::CODE + ln * 8) = code;
+      if ((ln & 3) == 0) *reinterpret_cast<uint32_t*>(part + P * L::CODE + off * L::SCALE + ln) = s8;
+    }
   }
-  // scale bytes of the head: 4 groups a word, collected in the first of each four lanes
-  uint32_t sw = s8 << (8 * (grp & 3));
-  sw |= __shfl_xor_sync(0xffffffffu, sw, 1);
-  sw |= __shfl_xor_sync(0xffffffffu, sw, 2);
-  if (!store) return;
-  const int64_t page = slot / P;
-  const int off = (int)(slot % P);
-  uint8_t* block = c.data + page * c.page_stride + (int64_t)h * c.head_stride;
-  *reinterpret_cast<uint2*>(block + (kv ? L::v_code(P) : 0) + off * L::CODE + grp * 8) = make_uint2(w[0], w[1]);
-  if ((grp & 3) == 0)
-    *reinterpret_cast<uint32_t*>(block + (kv ? L::v_scale(P) : L::k_scale(P)) + off * L::SCALE + grp) = sw;
 }
 
-// ---- gather ------------------------------------------------------------------
-template <typename T, int D, bool VEC>
+// 8 values from their codes and scale byte: code * scale is exact in fp16.
+template <typename T>
+CEK_DEVICE uint4 values8(uint32_t code, uint32_t s8, float g) {
+  const uint32_t s = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(s8), 0, 0x1010);
+  const uint32_t p[4] = {hmul2(e2m1x2_to_f16x2<0>(code), s), hmul2(e2m1x2_to_f16x2<1>(code), s),
+                         hmul2(e2m1x2_to_f16x2<2>(code), s), hmul2(e2m1x2_to_f16x2<3>(code), s)};
+  uint32_t o[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack2<__half>(p[j]);
+    o[j] = pack2<T>(__fmul_rn(f.x, g), __fmul_rn(f.y, g));
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <typename T, int D, bool VEC, int U>
 __global__ void __launch_bounds__(256)
-gather_kernel(Cache c, const int64_t* __restrict__ slots, T* __restrict__ key, T* __restrict__ value, int P,
-              int64_t groups, int64_t kts, int64_t khs, int64_t vts, int64_t vhs) {
+gather_kernel(Cache c, const int64_t* __restrict__ slots, T* __restrict__ key, T* __restrict__ value, int shift,
+              uint32_t units, const Divisor heads, int64_t kts, int64_t khs, int64_t vts, int64_t vhs) {
   using L = Layout<D>;
-  constexpr int GP = D / 16;
+  constexpr int LANES = D / 8, PER = 256 / LANES;
+  const int P = 1 << shift;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (id >= groups) return;
-  const int grp = (int)(id % GP);
-  const int64_t head_row = id / GP;
-  const int h = (int)(head_row % c.heads);
-  const int64_t r = head_row / c.heads;
-  const int kv = (int)(r & 1);
-  const int64_t t = r >> 1;
-  const int64_t slot = slots[t];
-  uint2 w = make_uint2(0u, 0u);
-  float s = 0.f;
-  if (slot >= 0 && slot < (int64_t)c.num_pages * P) {
-    const uint8_t* block = c.data + (slot / P) * c.page_stride + (int64_t)h * c.head_stride;
-    const int off = (int)(slot % P);
-    w = *reinterpret_cast<const uint2*>(block + (kv ? L::v_code(P) : 0) + off * L::CODE + grp * 8);
-    s = e4m3_to_f32(block[(kv ? L::v_scale(P) : L::k_scale(P)) + off * L::SCALE + grp]);
-  }
-  const float g = c.scales[kv * c.heads + h];
-  const uint32_t pr[8] = {e2m1x2_to_f16x2<0>(w.x), e2m1x2_to_f16x2<1>(w.x), e2m1x2_to_f16x2<2>(w.x),
-                          e2m1x2_to_f16x2<3>(w.x), e2m1x2_to_f16x2<0>(w.y), e2m1x2_to_f16x2<1>(w.y),
-                          e2m1x2_to_f16x2<2>(w.y), e2m1x2_to_f16x2<3>(w.y)};
-  uint32_t o[8];
+  const int ln = threadIdx.x % LANES;
+  const uint32_t u0 = blockIdx.x * (PER * U) + threadIdx.x / LANES;
+  int64_t slot[U];
+  int2 n[U];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = unpack2<__half>(pr[i]);
-    o[i] = pack2<T>(__fmul_rn(f.x * s, g), __fmul_rn(f.y * s, g));
+  for (int i = 0; i < U; ++i) {
+    n[i] = token_head(min(u0 + i * PER, units - 1), heads);
+    slot[i] = slots[n[i].x];
   }
-  T* dst = (kv ? value + t * vts + h * vhs : key + t * kts + h * khs) + grp * 16;
-  if constexpr (VEC) {
-    reinterpret_cast<uint4*>(dst)[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    reinterpret_cast<uint4*>(dst)[1] = make_uint4(o[4], o[5], o[6], o[7]);
-  } else {
-    const T* e = reinterpret_cast<const T*>(o);
+  uint32_t kc[U], vc[U], ks[U], vs[U];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) dst[i] = e[i];
+  for (int i = 0; i < U; ++i) {
+    kc[i] = vc[i] = ks[i] = vs[i] = 0;
+    if (slot[i] < 0 || slot[i] >= (int64_t)c.num_pages << shift) continue;
+    const uint8_t* block = c.data + (slot[i] >> shift) * c.page_stride + (int64_t)n[i].y * c.head_stride;
+    const int off = (int)slot[i] & (P - 1), code = off * L::CODE + ln * 4, sca = P * L::CODE + off * L::SCALE + (ln >> 1);
+    kc[i] = __ldg(reinterpret_cast<const uint32_t*>(block + code));
+    ks[i] = __ldg(block + sca);
+    vc[i] = __ldg(reinterpret_cast<const uint32_t*>(block + L::v_code(P) + code));
+    vs[i] = __ldg(block + L::v_code(P) + sca);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (u0 + i * PER >= units) continue;
+    store8<T, VEC>(key + (int64_t)n[i].x * kts + n[i].y * khs + ln * 8, values8<T>(kc[i], ks[i], c.scales[n[i].y]));
+    store8<T, VEC>(value + (int64_t)n[i].x * vts + n[i].y * vhs + ln * 8,
+                   values8<T>(vc[i], vs[i], c.scales[c.heads + n[i].y]));
   }
 }
 
 // ---- page plan -----------------------------------------------------------------
-// One cluster of up to 8 CTAs.  Every CTA scans the request lengths by itself
+// One cluster of up to 16 CTAs, one small CTA for a step of few tokens.  Every CTA scans the request lengths by itself
 // (a block scan of two sums; requests <= 4096), the cluster's barrier then
 // separates the last read of context_lens and free_count from the first write
 // of seq_lens and free_count_out (they may be the same arrays), and the CTAs
 // share the table entries and the tokens.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanTokensPerCta = 2048;
+constexpr int kPlanBatch = 4;
 
-CEK_DEVICE int pages_of(int tokens, int P) { return (int)(((int64_t)tokens + P - 1) / P); }
+CEK_DEVICE int pages_of(int tokens, const Divisor& P) {
+  const uint32_t full = divide((uint32_t)tokens, P);
+  return (int)(full + (full * P.d != (uint32_t)tokens));
+}
+
+// For N ascending searches at once: the last i in [0, n) with a[i] <= x, their
+// shared-memory loads in flight together.  a[0] <= x.
+template <int N>
+CEK_DEVICE void last_not_above(const int32_t* a, int n, const int (&x)[N], int (&at)[N]) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) at[k] = 0;
+  for (int step = 1 << (31 - __clz(n)); step > 0; step >>= 1) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (at[k] + step < n && a[at[k] + step] <= x[k]) at[k] += step;
+  }
+}
 
 __global__ void __launch_bounds__(kPlanThreads)
 plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens, int32_t* block_table,
             const int32_t* __restrict__ free_pages, const int32_t* free_count, int32_t* __restrict__ query_start,
             int32_t* seq_lens, int32_t* free_count_out, int64_t* __restrict__ positions, int64_t* __restrict__ slots,
-            int B, int W, int64_t table_stride, int pool, int64_t tokens, int P) {
+            int B, int W, int64_t table_stride, int pool, int64_t tokens, const Divisor P) {
   extern __shared__ int32_t sm[];
   int32_t* start = sm;               // [B + 1] first token of each request
-  int32_t* taken = sm + B + 1;       // [B] pages taken before request i; negative: refused
-  int32_t* ctx = sm + 2 * B + 1;     // [B]
+  int32_t* asked = sm + B + 1;       // [B + 1] pages asked for before each request
+  int32_t* ctx = sm + 2 * B + 2;     // [B] tokens that its pages hold; their complement (negative) if refused
   __shared__ int2 warp_sums[32];
   __shared__ int carry_q, carry_n, granted_pages;
   pdl_launch_dependents();
@@ -163,8 +250,8 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
   if (tid == 0) carry_q = carry_n = granted_pages = 0;
   const int avail = min(max(*free_count, 0), pool);
-  __syncthreads();
-  for (int b0 = 0; b0 < B; b0 += kPlanThreads) {
+  const int threads = blockDim.x, warps = threads >> 5;
+  for (int b0 = 0; b0 < B; b0 += threads) {
     const int i = b0 + tid;
     int q = 0, c = -1, need = 0;
     bool fits = false;
@@ -172,7 +259,7 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
       q = max(query_lens[i], 0);
       c = context_lens[i];
       if (c >= 0) {
-        const int have = pages_of(c, P), all = (int)(((int64_t)c + q + P - 1) / P);
+        const int have = pages_of(c, P), all = pages_of(c + q, P);
         fits = all <= W;
         need = fits ? all - have : 0;
       }
@@ -186,13 +273,13 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
     if (lane == 31) warp_sums[warp] = make_int2(sq, sn);
     __syncthreads();
     if (warp == 0) {
-      int2 v = warp_sums[lane];
+      int2 v = lane < warps ? warp_sums[lane] : make_int2(0, 0);
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int a = __shfl_up_sync(0xffffffffu, v.x, o), b = __shfl_up_sync(0xffffffffu, v.y, o);
         if (lane >= o) { v.x += a; v.y += b; }
       }
-      warp_sums[lane] = v;
+      if (lane < warps) warp_sums[lane] = v;
     }
     __syncthreads();
     if (warp > 0) { sq += warp_sums[warp - 1].x; sn += warp_sums[warp - 1].y; }
@@ -201,54 +288,64 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
     if (i < B) {
       const bool granted = fits && (need == 0 || sn <= avail);
       start[i] = sq - q;
-      taken[i] = granted ? sn - need : -1;
-      ctx[i] = c;
+      asked[i] = sn - need;
+      ctx[i] = granted ? c : c < 0 ? c : ~c;
       if (granted && need > 0) atomicMax(&granted_pages, sn);  // a maximum: the order does not matter
     }
     __syncthreads();
-    if (tid == kPlanThreads - 1) { carry_q = sq; carry_n = sn; }
+    if (tid == threads - 1) { carry_q = sq; carry_n = sn; }
     __syncthreads();
   }
-  if (tid == 0) start[B] = carry_q;
+  if (tid == 0) {
+    start[B] = carry_q;
+    asked[B] = carry_n;
+  }
   // all of the cluster has read context_lens and free_count
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
   __syncthreads();
-  const int stride = (int)ctas * kPlanThreads, gid = (int)rank * kPlanThreads + tid;
+  const int stride = (int)ctas * threads, gid = (int)rank * threads + tid;
   if (gid == 0) free_count_out[0] = avail - granted_pages;
   for (int i = gid; i <= B; i += stride) {
     query_start[i] = start[i];
-    if (i < B) {
-      const int c = ctx[i];
-      seq_lens[i] = taken[i] >= 0 ? c + (start[i + 1] - start[i]) : (c < 0 ? c : ~c);
-    }
+    if (i < B) seq_lens[i] = ctx[i] >= 0 ? ctx[i] + (start[i + 1] - start[i]) : ctx[i];
   }
-  // new table entries: a warp per request
-  for (int i = gid >> 5; i < B; i += stride >> 5) {
-    if (taken[i] < 0) continue;
-    const int have = pages_of(ctx[i], P), need = pages_of(ctx[i] + (start[i + 1] - start[i]), P) - have;
-    for (int j = lane; j < need; j += 32)
-      block_table[(int64_t)i * table_stride + have + j] = free_pages[avail - 1 - (taken[i] + j)];
+  // new table entries: entry e of the line of all pages asked for
+  const int entries = B > 0 ? min(asked[B], avail) : 0;
+  for (int e = gid; e < entries; e += stride) {
+    const int x[1] = {e};
+    int at[1];
+    last_not_above<1>(asked, B, x, at);
+    const int i = at[0], c = ctx[i];
+    if (c >= 0) block_table[(int64_t)i * table_stride + pages_of(c, P) + e - asked[i]] = free_pages[avail - 1 - e];
   }
+  // tokens, kPlanBatch a thread at once
   const int total = start[B];
-  for (int64_t t = gid; t < tokens; t += stride) {
-    int64_t position = 0, slot = -1;
-    if (t < total) {
-      int lo = 0, hi = B - 1;  // the last request whose first token is not behind t
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (start[mid] <= (int)t) lo = mid; else hi = mid - 1;
-      }
-      const int c = ctx[lo], pos = (c < 0 ? ~c : c) + (int)t - start[lo];
-      position = pos;
-      if (taken[lo] >= 0) {
-        const int have = pages_of(c, P), pg = pos / P;
-        const int page = pg < have ? block_table[(int64_t)lo * table_stride + pg]
-                                   : free_pages[avail - 1 - (taken[lo] + pg - have)];
-        slot = (int64_t)page * P + pos % P;
+  constexpr int N = kPlanBatch;
+  for (int64_t t0 = gid; t0 < tokens; t0 += (int64_t)stride * N) {
+    int x[N], at[N];
+    int64_t slot[N], position[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = (int)min(t0 + (int64_t)k * stride, (int64_t)INT32_MAX);
+    if (B > 0) last_not_above<N>(start, B, x, at);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      slot[k] = -1;
+      position[k] = 0;
+      if (x[k] >= total || x[k] >= tokens) continue;
+      const int i = at[k], c = ctx[i], pos = (c < 0 ? ~c : c) + x[k] - start[i];
+      position[k] = pos;
+      if (c >= 0) {
+        const int have = pages_of(c, P), pg = (int)divide((uint32_t)pos, P);
+        const int page = pg < have ? block_table[(int64_t)i * table_stride + pg] : free_pages[avail - 1 - (asked[i] + pg - have)];
+        slot[k] = (int64_t)page * P.d + (pos - pg * (int)P.d);
       }
     }
-    positions[t] = position;
-    slots[t] = slot;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (x[k] < tokens) {
+        positions[x[k]] = position[k];
+        slots[x[k]] = slot[k];
+      }
   }
 }
 
@@ -273,17 +370,29 @@ extern "C" int cek_kv_plan(const int32_t* query_lens, const int32_t* context_len
   if (requests > 0 && (!query_lens || !context_lens || !seq_lens || (table_width > 0 && !block_table)))
     return CEK_ERR_INVALID_ARG;
   if ((tokens > 0 && (!positions || !slot_mapping)) || (pool_size > 0 && !free_pages)) return CEK_ERR_INVALID_ARG;
-  const int smem = (int)(sizeof(int32_t) * (3 * requests + 1));
+  const int smem = (int)(sizeof(int32_t) * (3 * requests + 2));
   static cek_host::DeviceSlots slots_attr;
   if (smem > 48 * 1024 - 1024 &&
-      !cek_host::ensure_smem_attr(slots_attr, cek::kv4::plan_kernel, (int)sizeof(int32_t) * (3 * CEK_KV_PLAN_MAX_REQUESTS + 1)))
+      !cek_host::ensure_smem_attr(slots_attr, cek::kv4::plan_kernel, (int)sizeof(int32_t) * (3 * CEK_KV_PLAN_MAX_REQUESTS + 2)))
     return CEK_ERR_LAUNCH;
-  // CTAs by the tokens to write; a portable cluster has 8 at most
-  const int ctas = (int)std::min<int64_t>(8, std::max<int64_t>(1, (tokens + cek::kv4::kPlanTokensPerCta - 1) /
-                                                                      cek::kv4::kPlanTokensPerCta));
+  // CTAs by the tokens to write; above 8 a cluster is not portable, but this is one GPU's code
+  const int ctas = (int)std::min<int64_t>(16, std::max<int64_t>(1, (tokens + cek::kv4::kPlanTokensPerCta - 1) /
+                                                                       cek::kv4::kPlanTokensPerCta));
+  const int threads = requests <= 256 && tokens <= 1024 ? 256 : cek::kv4::kPlanThreads;
+  if (ctas > 8) {
+    static cek_host::DeviceSlots wide;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::atomic<int>* done = wide.at(dev);
+    if (!done || !done->load(std::memory_order_relaxed)) {
+      if (cudaFuncSetAttribute(cek::kv4::plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+        return CEK_ERR_LAUNCH;
+      if (done) done->store(1, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(cek::kv4::kPlanThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
@@ -296,7 +405,7 @@ extern "C" int cek_kv_plan(const int32_t* query_lens, const int32_t* context_len
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, cek::kv4::plan_kernel, query_lens, context_lens, block_table, free_pages, free_count,
                             query_start, seq_lens, free_count_out, positions, slot_mapping, (int)requests,
-                            (int)table_width, table_stride, (int)pool_size, tokens, (int)page_size) == cudaSuccess
+                            (int)table_width, table_stride, (int)pool_size, tokens, cek::kv4::Divisor((uint32_t)page_size)) == cudaSuccess
              ? CEK_OK
              : CEK_ERR_LAUNCH;
 }
@@ -314,35 +423,52 @@ int token_args(const void* key, const void* value, const int64_t* slots, const c
   if (tokens < 0 || (dtype != CEK_F16 && dtype != CEK_BF16)) return CEK_ERR_INVALID_ARG;
   if (tokens == 0) return CEK_OK;
   if (!key || !value || !slots) return CEK_ERR_INVALID_ARG;
-  if (tokens * 2 * cache->kv_heads * (cache->head_dim / 16) > (int64_t)INT32_MAX * 256) return CEK_ERR_INVALID_ARG;
+  if (tokens > INT32_MAX) return CEK_ERR_INVALID_ARG;
   *done = false;
   return CEK_OK;
 }
 }  // namespace
 
-#define CEK_KV4_DISPATCH(KERNEL, A0, A1, A2, A3)                                                                     \
+// Launches KERNEL on [tokens], in parts whose unit numbers stay below 2^31.
+#define CEK_KV4_DISPATCH(KERNEL, CHANNELS, A0, A1, A2, A3)                                                                    \
   do {                                                                                                               \
-    const int64_t groups = tokens * 2 * cache->kv_heads * (cache->head_dim / 16);                                    \
-    const dim3 grid((unsigned)((groups + 255) / 256)), block(256);                                                   \
+    const int64_t per = 256 / (cache->head_dim / CHANNELS), row = cache->kv_heads;                                      \
     cudaStream_t st = static_cast<cudaStream_t>(stream);                                                             \
     const bool vec = vec_ok(key, key_token_stride, key_head_stride) &&                                               \
                      vec_ok(value, value_token_stride, value_head_stride);                                           \
-    const int P = (int)cache->page_size;                                                                             \
-    auto go = [&](auto tag, auto dim, auto v) {                                                                      \
-      using T = decltype(tag);                                                                                       \
-      return cek_host::launch_pdl(cek::kv4::KERNEL<T, decltype(dim)::value, decltype(v)::value>, grid, block, 0, st, \
-                                  A0, A1, A2, A3, P, groups, key_token_stride, key_head_stride, value_token_stride,  \
-                                  value_head_stride);                                                                \
-    };                                                                                                               \
-    auto by_vec = [&](auto tag, auto dim) { return vec ? go(tag, dim, std::true_type{}) : go(tag, dim, std::false_type{}); }; \
-    auto by_dim = [&](auto tag) {                                                                                    \
-      switch (cache->head_dim) {                                                                                     \
-        case 64: return by_vec(tag, std::integral_constant<int, 64>{});                                              \
-        case 128: return by_vec(tag, std::integral_constant<int, 128>{});                                            \
-        default: return by_vec(tag, std::integral_constant<int, 256>{});                                             \
-      }                                                                                                              \
-    };                                                                                                               \
-    return dtype == CEK_F16 ? by_dim(__half{}) : by_dim(__nv_bfloat16{});                                            \
+    const cek::kv4::Divisor heads((uint32_t)cache->kv_heads);                                                          \
+    int shift = 0;                                                                                                   \
+    while ((1 << shift) < cache->page_size) ++shift;                                                                 \
+    const int64_t part = ((1ll << 31) - 4096) / row;                                                                 \
+    int rc = CEK_OK;                                                                                                 \
+    for (int64_t t0 = 0; t0 < tokens && rc == CEK_OK; t0 += part) {                                                  \
+      const uint32_t units = (uint32_t)(std::min(part, tokens - t0) * row);                                          \
+      /* one unit a thread until there are eight blocks an SM, then two */                                           \
+      const bool many = units > per * 8 * cek_host::sm_count();                                                      \
+      const dim3 grid((unsigned)((units + per * (many ? 2 : 1) - 1) / (per * (many ? 2 : 1)))), block(256);          \
+      auto go = [&](auto tag, auto dim, auto v) {                                                                    \
+        using T = decltype(tag);                                                                                     \
+        constexpr int D = decltype(dim)::value;                                                                      \
+        constexpr bool V = decltype(v)::value;                                                                       \
+        auto run = [&](auto kern) {                                                                                  \
+          return cek_host::launch_pdl(kern, grid, block, 0, st, A0, A1, A2, A3, shift, units, heads,                 \
+                                      key_token_stride, key_head_stride, value_token_stride, value_head_stride);     \
+        };                                                                                                           \
+        return many ? run(cek::kv4::KERNEL<T, D, V, 2>) : run(cek::kv4::KERNEL<T, D, V, 1>);                         \
+      };                                                                                                             \
+      auto by_vec = [&](auto tag, auto dim) {                                                                        \
+        return vec ? go(tag, dim, std::true_type{}) : go(tag, dim, std::false_type{});                               \
+      };                                                                                                             \
+      auto by_dim = [&](auto tag) {                                                                                  \
+        switch (cache->head_dim) {                                                                                   \
+          case 64: return by_vec(tag, std::integral_constant<int, 64>{});                                            \
+          case 128: return by_vec(tag, std::integral_constant<int, 128>{});                                          \
+          default: return by_vec(tag, std::integral_constant<int, 256>{});                                           \
+        }                                                                                                            \
+      };                                                                                                             \
+      rc = dtype == CEK_F16 ? by_dim(__half{}) : by_dim(__nv_bfloat16{});                                            \
+    }                                                                                                                \
+    return rc;                                                                                                       \
   } while (0)
 
 extern "C" int cek_kv4_append(const void* key, const void* value, const int64_t* slot_mapping,
@@ -353,7 +479,8 @@ extern "C" int cek_kv4_append(const void* key, const void* value, const int64_t*
   const int s = token_args(key, value, slot_mapping, cache, tokens, dtype, &done);
   if (done) return s;
   const cek::kv4::Cache c = cek_host::kv4_cache(cache);
-  CEK_KV4_DISPATCH(append_kernel, static_cast<const T*>(key), static_cast<const T*>(value), slot_mapping, c);
+  CEK_KV4_DISPATCH(append_kernel, 16, static_cast<const T*>(key) + t0 * key_token_stride,
+                   static_cast<const T*>(value) + t0 * value_token_stride, slot_mapping + t0, c);
 }
 
 extern "C" int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, void* key, void* value, int64_t tokens,
@@ -363,5 +490,6 @@ extern "C" int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, 
   const int s = token_args(key, value, slots, cache, tokens, dtype, &done);
   if (done) return s;
   const cek::kv4::Cache c = cek_host::kv4_cache(cache);
-  CEK_KV4_DISPATCH(gather_kernel, c, slots, static_cast<T*>(key), static_cast<T*>(value));
+  CEK_KV4_DISPATCH(gather_kernel, 8, c, slots + t0, static_cast<T*>(key) + t0 * key_token_stride,
+                   static_cast<T*>(value) + t0 * value_token_stride);
 }
