@@ -92,6 +92,14 @@ CEK_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint3
       "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
+// One lane of a converged warp.  The warp stays together around it, so that
+// addresses and descriptors are warp-uniform for the compiler: issued from a
+// branch on the lane number the matrix instructions took twice as long.
+CEK_DEVICE bool elect() {
+  uint32_t p;
+  asm volatile("{ .reg .pred e; elect.sync _|e, 0xffffffff; selp.u32 %0, 1, 0, e; }" : "=r"(p));
+  return p != 0;
+}
 CEK_DEVICE void tmem_ld32(uint32_t addr, float* r) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile(
@@ -401,28 +409,38 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       }
     } else if (warp == 12) {
       // ---- matrix instructions
-      if (lane == 0 && n > 0) {
-        bool ok = wait(mbar::saddr(&q_full), 0, &abort_flag);
+      if (n > 0) {
+        bool ok = wait_warp(mbar::saddr(&q_full), 0, &abort_flag);
         auto qk = [&](int j, int st) {  // S = Q K^T into the stream's (tile's) buffer
           const uint32_t d = tmem + (NQ == 2 ? st : j & 1) * 128;
           const uint32_t a = s_q + st * (128 * D * 2), b = s_kv + ((2 * j) & 3) * C::SLOT;
+          if (elect()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            mma_ss(d, desc(a + (k >> 2) * (128 * 128) + (k & 3) * 32, 16), desc(b + (k >> 2) * (TK * 128) + (k & 3) * 32, 16),
-                   C::IDESC_QK, k > 0);
-          commit(mbar::saddr(&s_full[NQ == 2 ? st : j & 1]));
+            for (int k = 0; k < D / 16; ++k)
+              mma_ss(d, desc(a + (k >> 2) * (128 * 128) + (k & 3) * 32, 16), desc(b + (k >> 2) * (TK * 128) + (k & 3) * 32, 16),
+                     C::IDESC_QK, k > 0);
+            commit(mbar::saddr(&s_full[NQ == 2 ? st : j & 1]));
+          }
+          __syncwarp();
         };
         auto pv = [&](int j, int st) {  // O += P V
           const uint32_t d = tmem + C::O_COL + st * D, a = tmem + (NQ == 2 ? st : j & 1) * 128;
           const uint32_t b = s_kv + ((2 * j + 1) & 3) * C::SLOT;
+          if (elect()) {
 #pragma unroll
-          for (int k = 0; k < TK / 16; ++k)
-            mma_ts(d, a + k * 8, desc(b + k * 2048, TK * 128), C::IDESC_PV, j > 0 || k > 0);
-          commit(mbar::saddr(&o_done[st]));
+            for (int k = 0; k < TK / 16; ++k)
+              mma_ts(d, a + k * 8, desc(b + k * 2048, TK * 128), C::IDESC_PV, j > 0 || k > 0);
+            commit(mbar::saddr(&o_done[st]));
+          }
+          __syncwarp();
         };
-        auto kv_ready = [&](int i) { return wait(mbar::saddr(&kv_full[i & 3]), (i >> 2) & 1, &abort_flag); };
+        auto release = [&](int i) {  // slot i once all products issued so far are done
+          if (elect()) commit(mbar::saddr(&kv_empty[i & 3]));
+          __syncwarp();
+        };
+        auto kv_ready = [&](int i) { return wait_warp(mbar::saddr(&kv_full[i & 3]), (i >> 2) & 1, &abort_flag); };
         auto p_ready = [&](int j, int st) {
-          const bool r = wait(mbar::saddr(&p_full[NQ == 2 ? st : j & 1]), NQ == 2 ? j & 1 : (j >> 1) & 1, &abort_flag);
+          const bool r = wait_warp(mbar::saddr(&p_full[NQ == 2 ? st : j & 1]), NQ == 2 ? j & 1 : (j >> 1) & 1, &abort_flag);
           fence_after();
           return r;
         };
@@ -430,7 +448,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         if (ok) {
           fence_after();
           for (int st = 0; st < NQ; ++st) qk(0, st);
-          commit(mbar::saddr(&kv_empty[0]));
+          release(0);
         }
         for (int j = 0; j < n && ok; ++j) {
           if constexpr (NQ == 2) {
@@ -438,13 +456,13 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
               ok = (st == 1 || kv_ready(2 * j + 1)) && p_ready(j, st);
               if (!ok) break;
               pv(j, st);
-              if (st == 1) commit(mbar::saddr(&kv_empty[(2 * j + 1) & 3]));
+              if (st == 1) release(2 * j + 1);
               if (j + 1 < n) {
                 if (st == 0) ok = kv_ready(2 * j + 2);
                 if (!ok) break;
                 fence_after();
                 qk(j + 1, st);
-                if (st == 1) commit(mbar::saddr(&kv_empty[(2 * j + 2) & 3]));
+                if (st == 1) release(2 * j + 2);
               }
             }
           } else {
@@ -453,15 +471,16 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
               if (!ok) break;
               fence_after();
               qk(j + 1, 0);
-              commit(mbar::saddr(&kv_empty[(2 * j + 2) & 3]));
+              release(2 * j + 2);
             }
             ok = kv_ready(2 * j + 1) && p_ready(j, 0);
             if (!ok) break;
             pv(j, 0);
-            commit(mbar::saddr(&kv_empty[(2 * j + 1) & 3]));
+            release(2 * j + 1);
           }
         }
-        commit(mbar::saddr(&drain));  // nothing of ours still runs when tensor memory is freed
+        if (elect()) commit(mbar::saddr(&drain));  // nothing of ours still runs when tensor memory is freed
+        __syncwarp();
         wait(mbar::saddr(&drain), 0, &abort_flag);
       }
     } else if (warp == 13) {
