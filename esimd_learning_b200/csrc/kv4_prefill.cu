@@ -8,7 +8,7 @@
 //    running maximum and sum, and writes P (fp16) over S;
 //  * converters: turn the codes of a page into the fp16 operands, exactly
 //    (kv4.cuh), straight into the 128-byte-swizzled layout that the matrix unit
-//    reads; a four-slot ring K(j), V(j), K(j+1), ...
+//    reads; a ring of slots K(j), V(j), K(j+1), ...
 //  * one warp copies pages (a bulk copy per page and half tile) into a raw ring;
 //  * one thread issues the matrix instructions: S = Q K^T with both operands in
 //    shared memory, O += P V with P in tensor memory and V read with keys as
@@ -42,7 +42,7 @@ namespace pf {
 constexpr float kShift = 6.f, kLazy = 8.f;
 constexpr int kThreads = 512;
 constexpr uint32_t kPolls = 1u << 24;
-constexpr int kRaw = 3;  // raw stages: halves of a tile
+constexpr int kSmem = 226 * 1024;  // dynamic shared memory of a CTA at most
 
 template <int D, int NQ>
 struct Cfg {
@@ -50,7 +50,11 @@ struct Cfg {
   static constexpr int RK = TK / 2;                       // keys of a raw stage
   static constexpr int ROWS = NQ * 128;
   static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2, RAW = Layout<D>::bytes(RK);
-  static constexpr int SMEM = Q_BYTES + 4 * SLOT + kRaw * RAW + 1024;
+  static constexpr int SLOTS = 4;                         // converted K and V tiles
+  // raw stages: what is left, 8 at most.  With 3 the wait for pages cost a third of a
+  // memory-bound call's time
+  static constexpr int RAW_ROOM = (kSmem - 1024 - Q_BYTES - SLOTS * SLOT) / RAW, RAWS = RAW_ROOM < 8 ? RAW_ROOM : 8;
+  static constexpr int SMEM = Q_BYTES + SLOTS * SLOT + RAWS * RAW + 1024;
   static constexpr int CONV_WARPS = NQ == 2 ? 4 : 8;      // warps 8..11, or 4..11
   static constexpr int O_COL = 256;
   static constexpr uint32_t IDESC_QK = (1u << 4) | (uint32_t(TK >> 3) << 17) | (8u << 24);
@@ -162,8 +166,9 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   constexpr int TK = C::TK, RK = C::RK, ROWS = C::ROWS, GP = D / 16;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (mbar::saddr(smem_raw) + 1023u) & ~1023u;
-  const uint32_t s_q = sbase, s_kv = sbase + C::Q_BYTES, s_rw = s_kv + 4 * C::SLOT;
-  __shared__ __align__(8) uint64_t raw_full[kRaw], raw_empty[kRaw], kv_full[4], kv_empty[4], s_full[2], p_full[2], o_done[2],
+  const uint32_t s_q = sbase, s_kv = sbase + C::Q_BYTES, s_rw = s_kv + C::SLOTS * C::SLOT;
+  constexpr int kRaw = C::RAWS, kSlots = C::SLOTS;
+  __shared__ __align__(8) uint64_t raw_full[kRaw], raw_empty[kRaw], kv_full[kSlots], kv_empty[kSlots], s_full[2], p_full[2], o_done[2],
       q_full, drain;
   __shared__ uint32_t tmem_sh;
   __shared__ volatile int abort_flag;
@@ -176,7 +181,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       mbar::init(mbar::saddr(&raw_full[i]), 1);
       mbar::init(mbar::saddr(&raw_empty[i]), C::CONV_WARPS);
     }
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       mbar::init(mbar::saddr(&kv_full[i]), C::CONV_WARPS);
       mbar::init(mbar::saddr(&kv_empty[i]), 1);
     }
@@ -363,8 +368,8 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       int raw = 0, slot = 0;  // stages and slots so far
       for (int j = 0; j < n && !bad; ++j) {
         for (int kv = 0; kv < 2 && !bad; ++kv, ++slot) {
-          if (!wait_warp(mbar::saddr(&kv_empty[slot & 3]), ((slot >> 2) & 1) ^ 1, &abort_flag)) { bad = true; break; }
-          const uint32_t out = s_kv + (slot & 3) * C::SLOT + at0;
+          if (!wait_warp(mbar::saddr(&kv_empty[slot % kSlots]), ((slot / kSlots) & 1) ^ 1, &abort_flag)) { bad = true; break; }
+          const uint32_t out = s_kv + (slot % kSlots) * C::SLOT + at0;
           for (int half = 0; half < 2; ++half) {
             const int rs = (raw + half) % kRaw;
             if (kv == 0 && !wait_warp(mbar::saddr(&raw_full[rs]), ((raw + half) / kRaw) & 1, &abort_flag)) { bad = true; break; }
@@ -403,7 +408,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           if (bad) break;
           proxy_fence();
           __syncwarp();
-          if (lane == 0) mbar::arrive(mbar::saddr(&kv_full[slot & 3]));
+          if (lane == 0) mbar::arrive(mbar::saddr(&kv_full[slot % kSlots]));
         }
         raw += 2;
       }
@@ -413,7 +418,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         bool ok = wait_warp(mbar::saddr(&q_full), 0, &abort_flag);
         auto qk = [&](int j, int st) {  // S = Q K^T into the stream's (tile's) buffer
           const uint32_t d = tmem + (NQ == 2 ? st : j & 1) * 128;
-          const uint32_t a = s_q + st * (128 * D * 2), b = s_kv + ((2 * j) & 3) * C::SLOT;
+          const uint32_t a = s_q + st * (128 * D * 2), b = s_kv + ((2 * j) % kSlots) * C::SLOT;
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
@@ -425,7 +430,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         };
         auto pv = [&](int j, int st) {  // O += P V
           const uint32_t d = tmem + C::O_COL + st * D, a = tmem + (NQ == 2 ? st : j & 1) * 128;
-          const uint32_t b = s_kv + ((2 * j + 1) & 3) * C::SLOT;
+          const uint32_t b = s_kv + ((2 * j + 1) % kSlots) * C::SLOT;
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < TK / 16; ++k)
@@ -435,10 +440,10 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           __syncwarp();
         };
         auto release = [&](int i) {  // slot i once all products issued so far are done
-          if (elect()) commit(mbar::saddr(&kv_empty[i & 3]));
+          if (elect()) commit(mbar::saddr(&kv_empty[i % kSlots]));
           __syncwarp();
         };
-        auto kv_ready = [&](int i) { return wait_warp(mbar::saddr(&kv_full[i & 3]), (i >> 2) & 1, &abort_flag); };
+        auto kv_ready = [&](int i) { return wait_warp(mbar::saddr(&kv_full[i % kSlots]), (i / kSlots) & 1, &abort_flag); };
         auto p_ready = [&](int j, int st) {
           const bool r = wait_warp(mbar::saddr(&p_full[NQ == 2 ? st : j & 1]), NQ == 2 ? j & 1 : (j >> 1) & 1, &abort_flag);
           fence_after();
@@ -517,11 +522,11 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : vf / l;
     T* dst = static_cast<T*>(p.out) + (int64_t)(real ? tok : 0) * p.ots + (int64_t)(real ? head : 0) * p.ohs;
     float* part = p.partial + (int64_t)blockIdx.x * (ROWS * (D + 2));
-    if (splits > 1) {
+    if (splits > 1 && real) {
       part[x * 128 + rr] = m == -INFINITY ? m : m * c;
       part[ROWS + x * 128 + rr] = l;
-      part += 2 * ROWS + (x * 128 + rr) * D;
     }
+    part += 2 * ROWS + (x * 128 + rr) * D;
 #pragma unroll 1
     for (int i = 0; i < D; i += 32) {
       float o[32];
@@ -537,7 +542,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         o[q] *= inv;
         if ((nan_groups >> ((i + q) >> 4)) & 1) o[q] = __int_as_float(0x7fffffff);
       }
-      if (splits > 1) {
+      if (splits > 1 && real) {
 #pragma unroll
         for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(part + i + q) = make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]);
       } else if (real) {
@@ -554,41 +559,55 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Joins the splits of a row: one warp per row, D / 32 channels a lane.
+// Joins the splits of a row: four warps a row, each every fourth split, then the
+// four in order; D / 32 channels a lane.
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(128)
 attn_prefill_join_kernel(const AttnParams p, int row_blocks, int splits) {
   using C = Cfg<D, NQ>;
-  constexpr int ROWS = C::ROWS, E = D / 32;
+  constexpr int ROWS = C::ROWS, E = D / 32, SIZE = ROWS * (D + 2);
+  __shared__ float red[4][D], red_l[4];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+  const int b = blockIdx.z, h = blockIdx.y, row = blockIdx.x;
   const Request r = request_of<C::TK>(p, b);
   const int qi = row / p.group, tok = r.t0 + qi;
   if (row >= r.n * p.group || tok < 0 || tok >= p.tokens) return;
   const int rb = row / ROWS, col = row % ROWS;
   const int64_t item = ((int64_t)(row_blocks - 1 - rb) * p.requests + b) * p.cache.heads + h;
-  const float* part = p.partial + item * splits * (ROWS * (D + 2));
+  const float* part = p.partial + item * splits * SIZE;
   float top = -INFINITY;
-  for (int s = lane; s < splits; s += 32) top = fmaxf(top, part[(int64_t)s * (ROWS * (D + 2)) + col]);
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, part[(int64_t)s * SIZE + col]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.f : top;
   float l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float* q = part + (int64_t)s * (ROWS * (D + 2));
+#pragma unroll 8
+  for (int s = sub; s < splits; s += 4) {
+    const float* q = part + (int64_t)s * SIZE;
     const float w = ex2(q[col] - base);
     l += w * q[ROWS + col];
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] += w * q[2 * ROWS + col * D + lane * E + e];
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) red[sub][lane * E + e] = o[e];
+  if (lane == 0) red_l[sub] = l;
+  __syncthreads();
+  if (sub != 0) return;
+  l = red_l[0] + red_l[1] + red_l[2] + red_l[3];
   const float inv = l == 0.f ? 0.f : p.cache.scales[p.cache.heads + h] / l;
   T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(h * p.group + row - qi * p.group) * p.ohs + lane * E;
+  uint32_t u[E / 2];
 #pragma unroll
-  for (int e = 0; e < E; ++e) dst[e] = from_f32<T>(o[e] * inv);
+  for (int e = 0; e < E; ++e) o[e] = (red[0][lane * E + e] + red[1][lane * E + e]) + (red[2][lane * E + e] + red[3][lane * E + e]);
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) u[e] = pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+  if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = u[0];
+  else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
+  else *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 struct Plan {
@@ -619,7 +638,7 @@ int launch(const AttnParams& p, const Plan& r, cudaStream_t st) {
   int s = cek_host::launch_pdl(attn_prefill_kernel<T, D, NQ>, dim3((unsigned)blocks), dim3(kThreads), Cfg<D, NQ>::SMEM, st,
                                p, r.row_blocks, r.splits);
   if (s != CEK_OK || r.splits == 1) return s;
-  const dim3 grid((unsigned)(((int64_t)p.max_q * p.group + 3) / 4), (unsigned)p.cache.heads, (unsigned)p.requests);
+  const dim3 grid((unsigned)(p.max_q * p.group), (unsigned)p.cache.heads, (unsigned)p.requests);
   return cek_host::launch_pdl(attn_prefill_join_kernel<T, D, NQ>, grid, dim3(128), 0, st, p, r.row_blocks, r.splits);
 }
 template <typename T>
