@@ -114,16 +114,46 @@ struct Feeder {
   CEK_DEVICE int page_id(const AttnParams& p, int i) const {
     return ((int64_t)i << p.page_shift) < end ? min(max(__ldg(row + i), 0), p.cache.num_pages - 1) : 0;
   }
-  // Asks for the tile into `dst`; the bytes complete on `bar`.
-  CEK_DEVICE void ask(const AttnParams& p, uint32_t dst, uint32_t bar, int lane) {
-    using L = Layout<D>;
-    const int key0 = tile * TK;
-    const int first = key0 >> p.page_shift;
-    if (first >= window + 32) {
+  // Page numbers of the tile at key0 are at hand after this (32 % (TK / P) == 0).
+  CEK_DEVICE void look(const AttnParams& p, int key0, int lane) {
+    if ((key0 >> p.page_shift) >= window + 32) {
       window += 32;
       ids = ids_next;
       ids_next = page_id(p, window + 32 + lane);
     }
+  }
+  // Asks for the keys (part 0) or values (1) of the tile at key0.
+  CEK_DEVICE void ask_part(const AttnParams& p, uint32_t dst, uint32_t bar, int lane, int key0, int part) const {
+    using L = Layout<D>;
+    const int first = key0 >> p.page_shift;
+    if (p.P <= TK) {
+      const int pages = min(TK >> p.page_shift, max(0, (end - key0 + p.P - 1) >> p.page_shift));
+      const int id = __shfl_sync(0xffffffffu, ids, (first - window + lane) & 31);
+      const uint32_t bytes = (uint32_t)L::v_code(p.P);
+      if (lane == 0) mbar::arrive_expect_tx(bar, bytes * pages);
+      __syncwarp();
+      if (lane < pages)
+        mbar::bulk_g2s(dst + lane * bytes, base + (int64_t)id * p.cache.page_stride + part * bytes, bytes, bar);
+    } else {
+      const int id = __shfl_sync(0xffffffffu, ids, (first - window) & 31);
+      const int off = key0 & (p.P - 1);
+      const bool any = key0 < end;
+      if (lane == 0) mbar::arrive_expect_tx(bar, any ? (uint32_t)L::v_code(TK) : 0u);
+      __syncwarp();
+      if (any && lane < 2) {
+        const int width = lane ? L::SCALE : L::CODE;
+        const int src = part * L::v_code(p.P) + (lane ? L::k_scale(p.P) : 0) + off * width;
+        mbar::bulk_g2s(dst + (lane ? L::k_scale(TK) : 0), base + (int64_t)id * p.cache.page_stride + src,
+                       (uint32_t)(TK * width), bar);
+      }
+    }
+  }
+  // Asks for the tile, keys and values, into `dst`; the bytes complete on `bar`.
+  CEK_DEVICE void ask(const AttnParams& p, uint32_t dst, uint32_t bar, int lane) {
+    using L = Layout<D>;
+    const int key0 = tile * TK;
+    const int first = key0 >> p.page_shift;
+    look(p, key0, lane);
     if (p.P <= TK) {
       const int pages = min(TK >> p.page_shift, max(0, (end - key0 + p.P - 1) >> p.page_shift));
       const int id = __shfl_sync(0xffffffffu, ids, (first - window + lane) & 31);  // TK / P divides 32

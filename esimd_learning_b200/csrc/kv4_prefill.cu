@@ -9,7 +9,8 @@
 //  * converters: turn the codes of a page into the fp16 operands, exactly
 //    (kv4.cuh), straight into the 128-byte-swizzled layout that the matrix unit
 //    reads; a ring of slots K(j), V(j), K(j+1), ...
-//  * one warp copies pages (a bulk copy per page and half tile) into a raw ring;
+//  * one warp copies pages (a bulk copy per page, keys and values apart) into a raw
+//    ring, in the order in which the converters free it;
 //  * one thread issues the matrix instructions: S = Q K^T with both operands in
 //    shared memory, O += P V with P in tensor memory and V read with keys as
 //    the strided dimension, so V needs no transpose.
@@ -47,13 +48,11 @@ constexpr int kSmem = 226 * 1024;  // dynamic shared memory of a CTA at most
 template <int D, int NQ>
 struct Cfg {
   static constexpr int TK = D == 256 ? 64 : 128;
-  static constexpr int RK = TK / 2;                       // keys of a raw stage
-  static constexpr int ROWS = NQ * 128;
-  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2, RAW = Layout<D>::bytes(RK);
+    static constexpr int ROWS = NQ * 128;
+  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2, RAW = Layout<D>::v_code(TK);  // a raw stage: a tile's keys or values
   static constexpr int SLOTS = 4;                         // converted K and V tiles
-  // raw stages: what is left, 8 at most.  With 3 the wait for pages cost a third of a
-  // memory-bound call's time
-  static constexpr int RAW_ROOM = (kSmem - 1024 - Q_BYTES - SLOTS * SLOT) / RAW, RAWS = RAW_ROOM < 8 ? RAW_ROOM : 8;
+  // raw stages: what is left, 16 at most
+  static constexpr int RAW_ROOM = (kSmem - 1024 - Q_BYTES - SLOTS * SLOT) / RAW, RAWS = RAW_ROOM < 16 ? RAW_ROOM : 16;
   static constexpr int SMEM = Q_BYTES + SLOTS * SLOT + RAWS * RAW + 1024;
   static constexpr int CONV_WARPS = NQ == 2 ? 4 : 8;      // warps 8..11, or 4..11
   static constexpr int O_COL = 256;
@@ -163,13 +162,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   using C = Cfg<D, NQ>;
   using L = Layout<D>;
-  constexpr int TK = C::TK, RK = C::RK, ROWS = C::ROWS, GP = D / 16;
+  constexpr int TK = C::TK, ROWS = C::ROWS, GP = D / 16;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (mbar::saddr(smem_raw) + 1023u) & ~1023u;
   const uint32_t s_q = sbase, s_kv = sbase + C::Q_BYTES, s_rw = s_kv + C::SLOTS * C::SLOT;
   constexpr int kRaw = C::RAWS, kSlots = C::SLOTS;
   __shared__ __align__(8) uint64_t raw_full[kRaw], raw_empty[kRaw], kv_full[kSlots], kv_empty[kSlots], s_full[2], p_full[2], o_done[2],
       q_full, drain;
+  __shared__ float row_unscale[ROWS];
   __shared__ uint32_t tmem_sh;
   __shared__ volatile int abort_flag;
   __shared__ volatile uint32_t nan_seen;
@@ -224,39 +224,48 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   if (soft) {
     if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ---- Q: this thread's row, 16-byte chunk ch of 64-channel block cb at ch ^ (row & 7)
-    const T* src = static_cast<const T*>(p.q) + (int64_t)(real ? tok : 0) * p.qts + (int64_t)(real ? head : 0) * p.qhs;
-    const uint32_t dst = s_q + x * (128 * D * 2) + rr * 128;
-    float unscale = 1.f, up = 1.f;
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-      uint32_t mx = 0;
-      if (real) {
-#pragma unroll 4
-        for (int i = 0; i < D / 8; ++i) {
-          const uint4 v = reinterpret_cast<const uint4*>(src)[i];
-          mx = __vmaxu2(__vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
-                                 __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)), mx);
+    // ---- Q: the warp's 32 rows, whole rows at a time; 16-byte chunk ch of
+    // 64-channel block cb goes to ch ^ (row & 7)
+    constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows at a time
+    const int64_t own = real ? (int64_t)tok * p.qts + (int64_t)head * p.qhs : -1;
+    const int ch = lane % LPR;
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += 8 * RPI) {
+      uint4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, own, i0 + i * RPI + lane / LPR);
+        v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + ch * 8) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = (warp & 3) * 32 + i0 + i * RPI + lane / LPR;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          // as in the decode kernel: a power of two a row, exactly, into fp16's range
+          uint32_t mx = __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
+                                 __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
+          mx = max(mx & 0xFFFFu, mx >> 16);
+#pragma unroll
+          for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          const int e = (int)(mx >> 7);
+          const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
+          const float up = __int_as_float((127 + k) << 23);
+          if (ch == 0) row_unscale[x * 128 + r] = __int_as_float((127 - k) << 23);
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = unpack2<T>(u[q]);
+            u[q] = pack2<__half>(f.x * up, f.y * up);
+          }
         }
+        sts16(s_q + x * (128 * D * 2) + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[i].x, v[i].y,
+              v[i].z, v[i].w);
       }
-      mx = max(mx & 0xFFFFu, mx >> 16);
-      const int e = (int)(mx >> 7);  // as in the decode kernel: a power of two, exactly, into fp16's range
-      const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
-      up = __int_as_float((127 + k) << 23);
-      unscale = __int_as_float((127 - k) << 23);
-    }
-#pragma unroll 4
-    for (int i = 0; i < D / 8; ++i) {
-      uint4 v = real ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const float2 a = unpack2<T>(v.x), b = unpack2<T>(v.y), d = unpack2<T>(v.z), f = unpack2<T>(v.w);
-        v = make_uint4(pack2<__half>(a.x * up, a.y * up), pack2<__half>(b.x * up, b.y * up),
-                       pack2<__half>(d.x * up, d.y * up), pack2<__half>(f.x * up, f.y * up));
-      }
-      sts16(dst + (i >> 3) * (128 * 128) + (((i & 7) ^ (rr & 7)) << 4), v.x, v.y, v.z, v.w);
     }
     proxy_fence();
     __syncwarp();
     if (lane == 0) mbar::arrive(mbar::saddr(&q_full));
+    const float unscale = std::is_same<T, __nv_bfloat16>::value ? row_unscale[x * 128 + rr] : 1.f;
     // score -> log2 units; not zero, so that a masked -inf stays -inf
     c = fmaxf(p.scale_log2 * unscale * p.cache.scales[it.h], 1.2e-38f);
     int whi = hi, wlo = lo;  // keys that every row of the warp sees
@@ -345,16 +354,15 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < 12) {
       // ---- converters: thread items are 16-channel groups of a key, the same
-      // places in every half tile
-      constexpr int NTHR = C::CONV_WARPS * 32, ITEMS = RK * GP / NTHR;
+      // places in every tile
+      constexpr int NTHR = C::CONV_WARPS * 32, ITEMS = TK * GP / NTHR;
       const int ct = threadIdx.x - (12 - C::CONV_WARPS) * 32;
-      const int BP = min(p.P, RK);
-      const uint32_t v_part = L::v_code(BP);
+      const int BP = min(p.P, TK);
       uint32_t from[ITEMS], from_s[ITEMS];
 #pragma unroll
       for (int e = 0; e < ITEMS; ++e) {
         const int key = (ct + e * NTHR) / GP, grp = (ct + e * NTHR) % GP, in = key & (BP - 1);
-        const uint32_t blk = (uint32_t)(key / BP) * L::bytes(BP);
+        const uint32_t blk = (uint32_t)(key / BP) * L::v_code(BP);
         from[e] = blk + in * L::CODE + grp * 8;
         from_s[e] = blk + L::k_scale(BP) + in * L::SCALE + grp;
       }
@@ -365,52 +373,46 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       const uint32_t flip = (grp >> 2) & 1;
       const uint32_t at0 = (grp >> 2) * (TK * 128) + row0 * 128 + ((((grp & 3) * 2 + flip) ^ (row0 & 7)) << 4);
       bool bad = false;
-      int raw = 0, slot = 0;  // stages and slots so far
+      int slot = 0;  // slots (and stages) so far: K and V of a tile in turn
       for (int j = 0; j < n && !bad; ++j) {
         for (int kv = 0; kv < 2 && !bad; ++kv, ++slot) {
           if (!wait_warp(mbar::saddr(&kv_empty[slot % kSlots]), ((slot / kSlots) & 1) ^ 1, &abort_flag)) { bad = true; break; }
           const uint32_t out = s_kv + (slot % kSlots) * C::SLOT + at0;
-          for (int half = 0; half < 2; ++half) {
-            const int rs = (raw + half) % kRaw;
-            if (kv == 0 && !wait_warp(mbar::saddr(&raw_full[rs]), ((raw + half) / kRaw) & 1, &abort_flag)) { bad = true; break; }
-            const uint32_t stage = s_rw + rs * C::RAW + (kv ? v_part : 0);
-            const int key0 = (it.tile0 + j) * TK + half * RK + row0;
-            uint2 w[ITEMS];
-            uint32_t sc[ITEMS];
+          const int rs = slot % kRaw;
+          if (!wait_warp(mbar::saddr(&raw_full[rs]), (slot / kRaw) & 1, &abort_flag)) { bad = true; break; }
+          const uint32_t stage = s_rw + rs * C::RAW;
+          uint2 w[ITEMS];
+          uint32_t sc[ITEMS];
+#pragma unroll
+          for (int e = 0; e < ITEMS; ++e) {
+            w[e] = lds_u64(stage + from[e]);
+            sc[e] = lds_u8(stage + from_s[e]);
+          }
+          if (kv) {
+            // slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
+            const int key0 = (it.tile0 + j) * TK + row0;
 #pragma unroll
             for (int e = 0; e < ITEMS; ++e) {
-              w[e] = lds_u64(stage + from[e]);
-              sc[e] = lds_u8(stage + from_s[e]);
-            }
-            if (kv) {
-              // slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
-#pragma unroll
-              for (int e = 0; e < ITEMS; ++e) {
-                if (key0 + e * (NTHR / GP) >= it.limit) sc[e] = 0;
-                if ((sc[e] & 0x7F) == 0x7F) { nan_seen = 1; sc[e] = 0; }
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < ITEMS; ++e) {
-              const uint32_t s2 = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(sc[e]), 0, 0x1010);
-              const uint32_t x = flip ? w[e].y : w[e].x, y = flip ? w[e].x : w[e].y;
-              const uint32_t dst = out + (half * RK + e * (NTHR / GP)) * 128;
-              sts16(dst, hmul2(e2m1x2_to_f16x2<0>(x), s2), hmul2(e2m1x2_to_f16x2<1>(x), s2),
-                    hmul2(e2m1x2_to_f16x2<2>(x), s2), hmul2(e2m1x2_to_f16x2<3>(x), s2));
-              sts16(dst ^ 16, hmul2(e2m1x2_to_f16x2<0>(y), s2), hmul2(e2m1x2_to_f16x2<1>(y), s2),
-                    hmul2(e2m1x2_to_f16x2<2>(y), s2), hmul2(e2m1x2_to_f16x2<3>(y), s2));
-            }
-            if (kv) {
-              __syncwarp();
-              if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));
+              if (key0 + e * (NTHR / GP) >= it.limit) sc[e] = 0;
+              if ((sc[e] & 0x7F) == 0x7F) { nan_seen = 1; sc[e] = 0; }
             }
           }
-          if (bad) break;
+#pragma unroll
+          for (int e = 0; e < ITEMS; ++e) {
+            const uint32_t s2 = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(sc[e]), 0, 0x1010);
+            const uint32_t x = flip ? w[e].y : w[e].x, y = flip ? w[e].x : w[e].y;
+            const uint32_t dst = out + e * (NTHR / GP) * 128;
+            sts16(dst, hmul2(e2m1x2_to_f16x2<0>(x), s2), hmul2(e2m1x2_to_f16x2<1>(x), s2),
+                  hmul2(e2m1x2_to_f16x2<2>(x), s2), hmul2(e2m1x2_to_f16x2<3>(x), s2));
+            sts16(dst ^ 16, hmul2(e2m1x2_to_f16x2<0>(y), s2), hmul2(e2m1x2_to_f16x2<1>(y), s2),
+                  hmul2(e2m1x2_to_f16x2<2>(y), s2), hmul2(e2m1x2_to_f16x2<3>(y), s2));
+          }
+          __syncwarp();
+          if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));
           proxy_fence();
           __syncwarp();
           if (lane == 0) mbar::arrive(mbar::saddr(&kv_full[slot % kSlots]));
         }
-        raw += 2;
       }
     } else if (warp == 12) {
       // ---- matrix instructions
@@ -490,13 +492,15 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       }
     } else if (warp == 13) {
       // ---- pages
-      Feeder<D, RK> feed;
-      const int first = it.tile0 * 2, total = n * 2;
-      if (n > 0) feed.load(p, it.b, it.h, first, total, it.limit, lane);
+      Feeder<D, TK> feed;
+      const int total = n * 2;
+      if (n > 0) feed.load(p, it.b, it.h, it.tile0, n, it.limit, lane);
       int i = 0;
       for (; i < total; ++i) {
         if (!wait_warp(mbar::saddr(&raw_empty[i % kRaw]), ((i / kRaw) & 1) ^ 1, &abort_flag)) break;
-        feed.ask(p, s_rw + (i % kRaw) * C::RAW, mbar::saddr(&raw_full[i % kRaw]), lane);
+        const int key0 = (it.tile0 + (i >> 1)) * TK;
+        if ((i & 1) == 0) feed.look(p, key0, lane);
+        feed.ask_part(p, s_rw + (i % kRaw) * C::RAW, mbar::saddr(&raw_full[i % kRaw]), lane, key0, i & 1);
       }
       for (int a = i > kRaw ? i - kRaw : 0; a < i; ++a)  // no copy of ours is still landing
         wait(mbar::saddr(&raw_full[a % kRaw]), (a / kRaw) & 1, &abort_flag);
