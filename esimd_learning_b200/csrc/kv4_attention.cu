@@ -118,16 +118,25 @@ CEK_DEVICE void scan_requests(const AttnParams& p, int32_t* prefix, int32_t* war
   __syncthreads();
 }
 
-// Ranges of the line: CTA c has tiles [c S, (c + 1) S), its warps four near-equal parts.
+// Ranges of the line: CTA c has tiles [c S, (c + 1) S), its warps four near-equal
+// parts.  S is at least a tile a warp, so that a CTA's pieces of a long segment
+// become one in shared memory.  Short segments (at most a tile a warp, padded to
+// one length) are never cut: a CTA has one of them, or each of its warps whole ones.
 struct Ranges {
   int total, share;
-  CEK_DEVICE Ranges(int total_, int ctas) : total(total_), share(max(1, (total_ + ctas - 1) / ctas)) {}
+  CEK_DEVICE Ranges(int total_, int share_) : total(total_), share(share_) {}
+  CEK_DEVICE static int share_of(int total, int ctas, int pad) {
+    if (pad == 0) return max(kDecodeWarps, (total + ctas - 1) / ctas);
+    int segments = (total / pad + ctas - 1) / ctas;
+    if (segments > 1) segments = (segments + kDecodeWarps - 1) / kDecodeWarps * kDecodeWarps;
+    return max(1, segments) * pad;
+  }
   CEK_DEVICE int at(int cta, int warp) const { return min(total, cta * share + share * warp / kDecodeWarps); }
   CEK_DEVICE int cta_of(int tile) const { return tile / share; }
   // The whole CTA is inside the segment: its warps' pieces become one.
   CEK_DEVICE bool merged(int cta, int first, int end) const {
     const int a = at(cta, 0), b = at(cta, kDecodeWarps);
-    return a < b && first <= a && b <= end;
+    return a + 1 < b && first <= a && b <= end;
   }
   // Where the piece of a segment is kept: a warp has a slot for its first
   // segment and one for its last; a merged CTA uses its first warp's.
@@ -139,9 +148,8 @@ struct Ranges {
 // What the join has to know of a segment that starts in a warp's part and goes
 // beyond it (one a warp at most); rows = 0: none.  In front of the pieces.
 struct JoinItem {
-  int first, end, total;  // the segment's and all tiles
-  int t0, h, row0, rows;  // first token, kv head, the row block's first row, the kv head's rows
-  int pad;
+  int first, end, total, share;  // the segment's tiles, all tiles, a CTA's
+  int t0, h, row0, rows;         // first token, kv head, the row block's first row, the kv head's rows
 };
 
 CEK_DEVICE uint32_t movmatrix_t(uint32_t a) {
@@ -178,7 +186,7 @@ attn_decode_kernel(const AttnParams p) {
   }
   pdl_wait();
   scan_requests<TK, ROWS>(p, prefix, warp_sums);
-  const Ranges ranges(prefix[p.requests], (int)gridDim.x);
+  const Ranges ranges(prefix[p.requests], Ranges::share_of(prefix[p.requests], (int)gridDim.x, p.pad_tiles));
   const int from = ranges.at(blockIdx.x, warp), to = ranges.at(blockIdx.x, warp + 1);
   bool merge = false;  // the CTA is inside one segment
   if (ranges.at(blockIdx.x, 0) < ranges.total) {
@@ -319,6 +327,10 @@ attn_decode_kernel(const AttnParams p) {
         if (lane == 0) atomicAdd(&g_timeouts, 1ull);
       }
       dead = __any_sync(0xffffffffu, dead);
+      if (tile - s.first >= s.r.live) {  // padding
+        if (asked < to && !dead) ask();
+        continue;
+      }
       const uint32_t sb = ring + st * C::STAGE;
       const int key0 = (s.r.tile0 + tile - s.first) * TK;
 
@@ -537,7 +549,7 @@ attn_decode_kernel(const AttnParams p) {
     const bool mine = !merge && piece0 == s.first && stop == s.first + s.tiles;
     const float vf = p.cache.scales[p.cache.heads + s.h];
     if (p.partial && lane == 0 && piece0 == s.first && (merge ? s.first + s.tiles > ranges.at(blockIdx.x, kDecodeWarps) : !mine))
-      *item = {s.first, s.first + s.tiles, ranges.total, s.r.t0, s.h, s.rb * ROWS, rows, 0};
+      *item = {s.first, s.first + s.tiles, ranges.total, ranges.share, s.r.t0, s.h, s.rb * ROWS, rows};
     // the ring is free once this warp's only segment is done: a merged piece goes there
     float* piece = merge ? reinterpret_cast<float*>(smem + warp * C::STAGES * C::STAGE)
                          : pieces + (int64_t)ranges.slot(blockIdx.x, warp, s.first, false) * (ROWS * (D + 2));
@@ -627,20 +639,33 @@ attn_decode_kernel(const AttnParams p) {
 }
 
 // ---- joining the pieces of a segment --------------------------------------------
-// CTA (c, y) joins the segments that decode CTA c's warps have left it, rows 2y
-// and 2y + 1 of the block: four warps a row, each every fourth piece, then the
-// four in order.
-constexpr int kJoinWarps = 4, kJoinRows = 2;
+// CTA (c, y) joins the segments that decode CTA c's warps have left it.  Few
+// pieces (a batch: what two neighbours share): CTA (c, 0) alone, a warp a row.
+// Many (a long request): rows 2y and 2y + 1, four warps a row, each every fourth
+// piece, then the four in order.
+constexpr int kJoinWarps = 8, kJoinFew = 8, kJoinSub = 4, kJoinRows = kJoinWarps / kJoinSub;
+
+template <int D>
+struct Joined {
+  float m = -INFINITY, l = 0.f, o[D / 32] = {};
+  CEK_DEVICE void add(float mi, float li, const float (&oi)[D / 32]) {
+    const float top = fmaxf(m, mi), base = top == -INFINITY ? 0.f : top, keep = ex2(m - base), wt = ex2(mi - base);
+    l = l * keep + li * wt;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) o[e] = o[e] * keep + oi[e] * wt;
+    m = top;
+  }
+};
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(32 * kJoinWarps * kJoinRows)
+__global__ void __launch_bounds__(32 * kJoinWarps)
 attn_join_kernel(const AttnParams p, int ctas) {
   constexpr int ROWS = 8 * NT, E = D / 32, SLOT = ROWS * (D + 2);
   __shared__ JoinItem items[kDecodeWarps];
-  __shared__ float red[kJoinRows][kJoinWarps][D], red_l[kJoinRows][kJoinWarps];
+  __shared__ float red[kJoinRows][kJoinSub][D], red_l[kJoinRows][kJoinSub], red_m[kJoinRows][kJoinSub];
   pdl_launch_dependents();
   pdl_wait();
-  const int cta = blockIdx.x, lane = threadIdx.x & 31, sub = (threadIdx.x >> 5) % kJoinWarps;
-  const int jr = (threadIdx.x >> 5) / kJoinWarps, col = blockIdx.y * kJoinRows + jr;
+  const int cta = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr int WORDS = sizeof(JoinItem) / 4 * kDecodeWarps;
   const float* pieces = p.partial + (int64_t)ctas * WORDS;
   if (threadIdx.x < WORDS)
@@ -648,78 +673,80 @@ attn_join_kernel(const AttnParams p, int ctas) {
   __syncthreads();
   for (int w = 0; w < kDecodeWarps; ++w) {
     const JoinItem s = items[w];
-    if (s.row0 + (int)blockIdx.y * kJoinRows >= s.rows) continue;
-    const Ranges ranges(s.total, ctas);
-    const int c = s.row0 + col, qi = c / p.group, tok = s.t0 + qi;
-    const bool real = c < s.rows && tok >= 0 && tok < p.tokens;
+    if (s.rows == 0) continue;
+    const Ranges ranges(s.total, s.share);
     // pieces: warps of the first CTA, whole CTAs, warps of the last CTA
     const int c1 = ranges.cta_of(s.end - 1);
     const bool one0 = ranges.merged(cta, s.first, s.end), one1 = ranges.merged(c1, s.first, s.end);
     const int n0 = one0 ? 1 : kDecodeWarps, mid = max(0, c1 - cta - 1);
     const int count = n0 + mid + (c1 > cta ? (one1 ? 1 : kDecodeWarps) : 0);
+    const bool few = count <= kJoinFew;
+    if (few && blockIdx.y > 0) continue;
     auto slot_at = [&](int k) -> int {
+      if (k >= count) return -1;
       if (k >= n0 && k < n0 + mid) return ranges.slot(cta + 1 + k - n0, 0, s.first, true);
       const int kc = k < n0 ? cta : c1, kw = k < n0 ? k : k - n0 - mid;
       if (k < n0 ? one0 : one1) return ranges.slot(kc, 0, s.first, true);
       const int a = max(s.first, ranges.at(kc, kw)), b = min(s.end, ranges.at(kc, kw + 1));
       return a < b ? ranges.slot(kc, kw, s.first, false) : -1;
     };
-    float top = -INFINITY;
-    if (real)
-      for (int k = lane; k < count; k += 32) {
-        const int sl = slot_at(k);
-        if (sl >= 0) top = fmaxf(top, pieces[(int64_t)sl * SLOT + col]);
-      }
-    top = warp_max(top);
-    const float base = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o[E];
+    // pieces from, from + step, ... of a row, four in flight
+    auto collect = [&](Joined<D>& j, int col, int from, int step) {
+      constexpr int N = 4;
+      for (int k0 = from; k0 < count; k0 += N * step) {
+        float mi[N], li[N], oi[N][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.f;
-    if (real) {
-      for (int k0 = sub; k0 < count; k0 += 32 * kJoinWarps) {
-        // a piece a lane: its place and weight, then all of them in turn
-        const int mine = k0 + lane * kJoinWarps;
-        const int sl = mine < count ? slot_at(mine) : -1;
-        float wt = 0.f;
-        if (sl >= 0) {
-          wt = ex2(pieces[(int64_t)sl * SLOT + col] - base);
-          l += wt * pieces[(int64_t)sl * SLOT + ROWS + col];
+        for (int i = 0; i < N; ++i) {
+          const int sl = slot_at(k0 + i * step);
+          const float* q = pieces + (int64_t)max(sl, 0) * SLOT;
+          mi[i] = sl >= 0 ? q[col] : -INFINITY;
+          li[i] = sl >= 0 ? q[ROWS + col] : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) oi[i][e] = sl >= 0 ? q[2 * ROWS + col * D + lane * E + e] : 0.f;
         }
-        const int n = min(32, (count - k0 + kJoinWarps - 1) / kJoinWarps);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-          const int si = __shfl_sync(0xffffffffu, sl, i);
-          const float wi = __shfl_sync(0xffffffffu, wt, i);
-          if (si < 0) continue;
-          const float* q = pieces + (int64_t)si * SLOT + 2 * ROWS + col * D + lane * E;
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += wi * q[e];
-        }
+        for (int i = 0; i < N; ++i) j.add(mi[i], li[i], oi[i]);
       }
-    }
-    l = warp_sum(l);
-#pragma unroll
-    for (int e = 0; e < E; ++e) red[jr][sub][lane * E + e] = o[e];
-    if (lane == 0) red_l[jr][sub] = l;
-    __syncthreads();
-    if (sub == 0 && real) {
-      l = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < kJoinWarps; ++i) {
-        l += red_l[jr][i];
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += red[jr][i][lane * E + e];
-      }
-      const float inv = l == 0.f ? 0.f : p.cache.scales[p.cache.heads + s.h] / l;
+    };
+    auto write = [&](const Joined<D>& j, int c) {
+      const int qi = c / p.group, tok = s.t0 + qi;
+      if (c >= s.rows || tok < 0 || tok >= p.tokens) return;
+      const float inv = j.l == 0.f ? 0.f : p.cache.scales[p.cache.heads + s.h] / j.l;
       T* dst = static_cast<T*>(p.out) + (int64_t)tok * p.ots + (int64_t)(s.h * p.group + c - qi * p.group) * p.ohs + lane * E;
       uint32_t u[E / 2];
 #pragma unroll
-      for (int e = 0; e < E / 2; ++e) u[e] = pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+      for (int e = 0; e < E / 2; ++e) u[e] = pack2<T>(j.o[2 * e] * inv, j.o[2 * e + 1] * inv);
       if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = u[0];
       else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u[0], u[1]);
       else *reinterpret_cast<uint4*>(dst) = make_uint4(u[0], u[1], u[2], u[3]);
+    };
+    if (few) {
+      for (int col = warp; col < ROWS && s.row0 + col < s.rows; col += kJoinWarps) {
+        Joined<D> j;
+        collect(j, col, 0, 1);
+        write(j, s.row0 + col);
+      }
+      continue;
+    }
+    const int jr = warp / kJoinSub, sub = warp % kJoinSub, col = blockIdx.y * kJoinRows + jr;
+    Joined<D> j;
+    if (s.row0 + col < s.rows) collect(j, col, sub, kJoinSub);
+#pragma unroll
+    for (int e = 0; e < E; ++e) red[jr][sub][lane * E + e] = j.o[e];
+    if (lane == 0) {
+      red_l[jr][sub] = j.l;
+      red_m[jr][sub] = j.m;
+    }
+    __syncthreads();
+    if (sub == 0) {
+#pragma unroll
+      for (int i = 1; i < kJoinSub; ++i) {
+        float oi[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) oi[e] = red[jr][i][lane * E + e];
+        j.add(red_m[jr][i], red_l[jr][i], oi);
+      }
+      write(j, s.row0 + col);
     }
     __syncthreads();
   }
@@ -736,6 +763,7 @@ constexpr int64_t kDecodeRows = 16;  // rows of a kv head that the decode kernel
 
 struct DecodePlan {
   int nt, ctas;
+  int pad;              // tiles of a segment where all are short, else 0
   size_t smem;
   bool join;            // some segment may be in several pieces
   int64_t partial_bytes;
@@ -748,12 +776,13 @@ DecodePlan plan_decode_dn(int64_t requests, int64_t heads, int64_t group, int64_
   d.nt = NT;
   const int64_t req = std::min<int64_t>(requests, kMaxRequests);
   const int64_t segments = req * heads * ((max_q * group + 8 * NT - 1) / (8 * NT));
-  const int64_t tiles = (max_seq + C::TK - 1) / C::TK + 1;  // a window may start inside a tile
+  const int64_t tiles = std::max<int64_t>(1, (max_seq + C::TK - 1) / C::TK);
+  d.pad = tiles <= kDecodeWarps ? (int)tiles : 0;
   d.smem = (size_t)C::RING + sizeof(int32_t) * (req + 1);
   const int per_sm = (int)std::min<int64_t>(C::PER_SM, 233472 / (d.smem + 1024 + 512));  // 228 KB an SM, 1 KB a CTA reserved
   const int64_t most = (int64_t)std::max(1, per_sm) * cek_host::sm_count();
-  d.ctas = (int)std::min(most, segments >= most ? most : segments * tiles);
-  d.join = max_seq > C::TK;
+  d.ctas = (int)std::min(most, segments >= most ? most : segments * ((tiles + kDecodeWarps - 1) / kDecodeWarps));
+  d.join = d.pad == 0;
   d.partial_bytes = d.join ? (int64_t)kDecodeWarps * d.ctas * (sizeof(JoinItem) + 2 * 8 * NT * (D + 2) * sizeof(float)) : 0;
   return d;
 }
@@ -776,7 +805,7 @@ int launch_decode(const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
   int s = cek_host::launch_pdl(attn_decode_kernel<T, D, NT>, dim3(d.ctas), dim3(kDecodeThreads), d.smem, st, p);
   if (s != CEK_OK || !d.join) return s;
   return cek_host::launch_pdl(attn_join_kernel<T, D, NT>, dim3(d.ctas, 8 * NT / kJoinRows),
-                              dim3(32 * kJoinWarps * kJoinRows), 0, st, p, d.ctas);
+                              dim3(32 * kJoinWarps), 0, st, p, d.ctas);
 }
 template <typename T>
 int launch_decode_t(int64_t dim, const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
@@ -848,6 +877,7 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
     if (workspace_bytes < d.partial_bytes || (d.partial_bytes > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
     if (d.partial_bytes > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
     p.partial = d.join ? static_cast<float*>(workspace) : nullptr;
+    p.pad_tiles = d.pad;
     int rc = CEK_OK;
     for (int64_t b = 0; b < requests && rc == CEK_OK; b += kMaxRequests) {  // the prefix sums of a launch are bounded
       p.requests = (int)std::min<int64_t>(kMaxRequests, requests - b);

@@ -19,6 +19,7 @@ struct AttnParams {
   int max_q, max_seq, key_limit, window;  // key_limit: table_width * P
   float scale_log2;  // softmax_scale * log2(e)
   float* partial;    // pieces of split segments
+  int pad_tiles;     // decode: tiles that every request counts, 0: its own
 };
 
 // kv4_prefill.cu
@@ -30,7 +31,8 @@ bool prefill_timeouts(unsigned long long* count);
 struct Request {
   int t0, n;          // first token row, rows tokens (bounded)
   int pos0;           // position of the first token
-  int tile0, tiles;   // tiles of TK keys that any row sees (at least one if n > 0: it writes the zeros)
+  int tile0, live;    // tiles of TK keys that any row sees (at least one if n > 0: it writes the zeros)
+  int tiles;          // the same, or the length that all requests are padded to
   int end;            // keys behind it do not exist
 };
 template <int TK>
@@ -44,7 +46,8 @@ CEK_DEVICE Request request_of(const AttnParams& p, int b) {
   r.end = max(0, min(min(r.pos0 + r.n, p.max_seq), p.key_limit));
   const int lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
   r.tile0 = min(lo, r.end) / TK;
-  r.tiles = r.n > 0 ? max(1, (r.end + TK - 1) / TK - r.tile0) : 0;
+  r.live = r.n > 0 ? max(1, (r.end + TK - 1) / TK - r.tile0) : 0;
+  r.tiles = p.pad_tiles > 0 && r.n > 0 ? p.pad_tiles : r.live;
   return r;
 }
 
