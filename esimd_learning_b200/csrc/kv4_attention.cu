@@ -120,7 +120,7 @@ CEK_DEVICE void scan_requests(const AttnParams& p, int32_t* prefix, int32_t* war
 
 // Ranges of the line: CTA c has tiles [c S, (c + 1) S), its warps four near-equal
 // parts.  S is at least a tile a warp, so that a CTA's pieces of a long segment
-// become one in shared memory.  Short segments (at most a tile a warp, padded to
+// become one in shared memory.  Short segments (one or two tiles a warp, padded to
 // one length) are never cut: a CTA has one of them, or each of its warps whole ones.
 struct Ranges {
   int total, share;
@@ -777,11 +777,13 @@ DecodePlan plan_decode_dn(int64_t requests, int64_t heads, int64_t group, int64_
   const int64_t req = std::min<int64_t>(requests, kMaxRequests);
   const int64_t segments = req * heads * ((max_q * group + 8 * NT - 1) / (8 * NT));
   const int64_t tiles = std::max<int64_t>(1, (max_seq + C::TK - 1) / C::TK);
-  d.pad = tiles <= kDecodeWarps ? (int)tiles : 0;
   d.smem = (size_t)C::RING + sizeof(int32_t) * (req + 1);
   const int per_sm = (int)std::min<int64_t>(C::PER_SM, 233472 / (d.smem + 1024 + 512));  // 228 KB an SM, 1 KB a CTA reserved
   const int64_t most = (int64_t)std::max(1, per_sm) * cek_host::sm_count();
-  d.ctas = (int)std::min(most, segments >= most ? most : segments * ((tiles + kDecodeWarps - 1) / kDecodeWarps));
+  // A cut costs a second launch, 4 to 5 us: with a CTA for every segment, two tiles a warp
+  // (another 1.3 us) are cheaper; otherwise a warp takes whole segments of up to four.
+  d.pad = tiles <= (segments <= most ? 2 : 1) * kDecodeWarps ? (int)tiles : 0;
+  d.ctas = (int)std::min(most, segments >= most ? most : segments * (d.pad ? 1 : (tiles + kDecodeWarps - 1) / kDecodeWarps));
   d.join = d.pad == 0;
   d.partial_bytes = d.join ? (int64_t)kDecodeWarps * d.ctas * (sizeof(JoinItem) + 2 * 8 * NT * (D + 2) * sizeof(float)) : 0;
   return d;

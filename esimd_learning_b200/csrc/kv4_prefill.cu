@@ -227,18 +227,19 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     // ---- Q: the warp's 32 rows, whole rows at a time; 16-byte chunk ch of
     // 64-channel block cb goes to ch ^ (row & 7)
     constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows at a time
+    constexpr int FLY = 32 / RPI < 16 ? 32 / RPI : 16;  // loads in flight
     const int64_t own = real ? (int64_t)tok * p.qts + (int64_t)head * p.qhs : -1;
     const int ch = lane % LPR;
 #pragma unroll
-    for (int i0 = 0; i0 < 32; i0 += 8 * RPI) {
-      uint4 v[8];
+    for (int i0 = 0; i0 < 32; i0 += FLY * RPI) {
+      uint4 v[FLY];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < FLY; ++i) {
         const int64_t at = __shfl_sync(0xffffffffu, own, i0 + i * RPI + lane / LPR);
         v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + ch * 8) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < FLY; ++i) {
         const int r = (warp & 3) * 32 + i0 + i * RPI + lane / LPR;
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
           // as in the decode kernel: a power of two a row, exactly, into fp16's range
