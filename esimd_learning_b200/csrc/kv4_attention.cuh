@@ -125,12 +125,13 @@ struct Feeder {
       ids_next = page_id(p, window + 32 + lane);
     }
   }
-  // Asks for the keys (part 0) or values (1) of the tile at key0.
+  // Asks for the keys (part 0) or values (1) of N tokens at key0, within the tile looked at.
+  template <int N>
   CEK_DEVICE void ask_part(const AttnParams& p, uint32_t dst, uint32_t bar, int lane, int key0, int part) const {
     using L = Layout<D>;
     const int first = key0 >> p.page_shift;
-    if (p.P <= TK) {
-      const int pages = min(TK >> p.page_shift, max(0, (end - key0 + p.P - 1) >> p.page_shift));
+    if (p.P <= N) {
+      const int pages = min(N >> p.page_shift, max(0, (end - key0 + p.P - 1) >> p.page_shift));
       const int id = __shfl_sync(0xffffffffu, ids, (first - window + lane) & 31);
       const uint32_t bytes = (uint32_t)L::v_code(p.P);
       if (lane == 0) mbar::arrive_expect_tx(bar, bytes * pages);
@@ -141,13 +142,13 @@ struct Feeder {
       const int id = __shfl_sync(0xffffffffu, ids, (first - window) & 31);
       const int off = key0 & (p.P - 1);
       const bool any = key0 < end;
-      if (lane == 0) mbar::arrive_expect_tx(bar, any ? (uint32_t)L::v_code(TK) : 0u);
+      if (lane == 0) mbar::arrive_expect_tx(bar, any ? (uint32_t)L::v_code(N) : 0u);
       __syncwarp();
       if (any && lane < 2) {
         const int width = lane ? L::SCALE : L::CODE;
         const int src = part * L::v_code(p.P) + (lane ? L::k_scale(p.P) : 0) + off * width;
-        mbar::bulk_g2s(dst + (lane ? L::k_scale(TK) : 0), base + (int64_t)id * p.cache.page_stride + src,
-                       (uint32_t)(TK * width), bar);
+        mbar::bulk_g2s(dst + (lane ? L::k_scale(N) : 0), base + (int64_t)id * p.cache.page_stride + src,
+                       (uint32_t)(N * width), bar);
       }
     }
   }

@@ -45,20 +45,21 @@ constexpr int kThreads = 512;
 constexpr uint32_t kPolls = 1u << 24;
 constexpr int kSmem = 226 * 1024;  // dynamic shared memory of a CTA at most
 
-template <int D, int NQ>
+// CG CTAs share their K and V (a cluster; CG = 2 for D = 128, NQ = 2).
+template <int D, int NQ, int CG>
 struct Cfg {
   static constexpr int TK = D == 256 ? 64 : 128;
-    static constexpr int ROWS = NQ * 128;
-  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2, RAW = Layout<D>::v_code(TK);  // a raw stage: a tile's keys or values
+    static constexpr int ROWS = NQ * 128;                   // of a CTA; an item has CG of them
+  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2 / CG, RAW = Layout<D>::v_code(TK);  // a raw stage: a tile's keys or values
   static constexpr int SLOTS = 4;                         // converted K and V tiles
   // raw stages: what is left, 16 at most
   static constexpr int RAW_ROOM = (kSmem - 1024 - Q_BYTES - SLOTS * SLOT) / RAW, RAWS = RAW_ROOM < 16 ? RAW_ROOM : 16;
   static constexpr int SMEM = Q_BYTES + SLOTS * SLOT + RAWS * RAW + 1024;
   static constexpr int CONV_WARPS = NQ == 2 ? 4 : 8;      // warps 8..11, or 4..11
   static constexpr int O_COL = 256;
-  static constexpr uint32_t IDESC_QK = (1u << 4) | (uint32_t(TK >> 3) << 17) | (8u << 24);
+  static constexpr uint32_t IDESC_QK = (1u << 4) | (uint32_t(TK >> 3) << 17) | (uint32_t(8 * CG) << 24);
   // bit 16: B (V) has its N dimension contiguous
-  static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (8u << 24);
+  static constexpr uint32_t IDESC_PV = (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(8 * CG) << 24);
 };
 
 CEK_DEVICE bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
@@ -74,10 +75,51 @@ CEK_DEVICE bool wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
 CEK_DEVICE bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, wait(bar, parity, abort_flag));
 }
+CEK_DEVICE uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
 CEK_DEVICE void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 CEK_DEVICE void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives on `bar` of every CTA of the group when the products issued so far are done.
+template <int CG>
 CEK_DEVICE void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+}
+// Arrives on the leading CTA's `bar` (this CTA's, where it is alone).  What the
+// arrival announces is complete before it: converted tiles by fence.proxy.async,
+// P by tcgen05.wait::st and fence::before_thread_sync.  It need not order more
+// (release at cluster scope cost some 900 cycles each time, twice the products).
+template <int CG>
+CEK_DEVICE void arrive_lead(uint32_t bar) {
+  if constexpr (CG == 1)
+    mbar::arrive(bar);
+  else
+    asm volatile(
+        "{ .reg .b32 r; mapa.shared::cluster.u32 r, %0, 0; mbarrier.arrive.shared::cluster.b64 _, [r]; }" ::"r"(bar)
+        : "memory");
+}
+// Stores to the same place in every CTA of the group.
+template <int CG>
+CEK_DEVICE void store_all(uint32_t addr, uint32_t v) {
+#pragma unroll
+  for (int r = 0; r < CG; ++r)
+    asm volatile("{ .reg .b32 a; mapa.shared::cluster.u32 a, %0, %1; st.shared::cluster.u32 [a], %2; }" ::"r"(addr), "r"(r), "r"(v)
+                 : "memory");
+}
+// A barrier of all threads of the group, memory included.
+template <int CG>
+CEK_DEVICE void sync_group() {
+  if constexpr (CG == 1)
+    __syncthreads();
+  else
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart;
 // `lead` is the distance of 64-element blocks where those are contiguous (V).
@@ -85,15 +127,23 @@ CEK_DEVICE uint64_t desc(uint32_t addr, uint32_t lead) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+template <int CG>
 CEK_DEVICE void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
+template <int CG>
 CEK_DEVICE void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
 // One lane of a converged warp.  The warp stays together around it, so that
 // addresses and descriptors are warp-uniform for the compiler: issued from a
@@ -135,9 +185,9 @@ struct Item {
   int tile0, tiles;    // of this split
   int limit;           // no row of the block sees a key at or past it
 };
-template <int TK, int ROWS>
+template <int TK, int ROWS, int CG>
 CEK_DEVICE bool item_of(const AttnParams& p, int row_blocks, int splits, Item& it) {
-  int64_t id = blockIdx.x;
+  int64_t id = blockIdx.x / CG;
   it.split = (int)(id % splits);
   id /= splits;
   it.h = (int)(id % p.cache.heads);
@@ -157,12 +207,13 @@ CEK_DEVICE bool item_of(const AttnParams& p, int row_blocks, int splits, Item& i
   return true;
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
-  using C = Cfg<D, NQ>;
+  using C = Cfg<D, NQ, CG>;
   using L = Layout<D>;
   constexpr int TK = C::TK, ROWS = C::ROWS, GP = D / 16;
+  static_assert(CG == 1 || (D == 128 && NQ == 2), "a pair halves V by 64 channels");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (mbar::saddr(smem_raw) + 1023u) & ~1023u;
   const uint32_t s_q = sbase, s_kv = sbase + C::Q_BYTES, s_rw = s_kv + C::SLOTS * C::SLOT;
@@ -182,15 +233,15 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       mbar::init(mbar::saddr(&raw_empty[i]), C::CONV_WARPS);
     }
     for (int i = 0; i < kSlots; ++i) {
-      mbar::init(mbar::saddr(&kv_full[i]), C::CONV_WARPS);
+      mbar::init(mbar::saddr(&kv_full[i]), CG * C::CONV_WARPS);
       mbar::init(mbar::saddr(&kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar::init(mbar::saddr(&s_full[i]), 1);
-      mbar::init(mbar::saddr(&p_full[i]), 4);
+      mbar::init(mbar::saddr(&p_full[i]), CG * 4);
       mbar::init(mbar::saddr(&o_done[i]), 1);
     }
-    mbar::init(mbar::saddr(&q_full), 4 * NQ);
+    mbar::init(mbar::saddr(&q_full), CG * 4 * NQ);
     mbar::init(mbar::saddr(&drain), 1);
     abort_flag = 0;
     nan_seen = 0;
@@ -198,13 +249,19 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   }
   pdl_wait();
   Item it;
-  if (!item_of<TK, ROWS>(p, row_blocks, splits, it)) return;  // the whole block
+  if (!item_of<TK, CG * ROWS, CG>(p, row_blocks, splits, it)) return;  // the whole group
+  const uint32_t rank = CG == 1 ? 0 : cta_rank();
   if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mbar::saddr(&tmem_sh)), "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mbar::saddr(&tmem_sh)), "r"(512));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mbar::saddr(&tmem_sh)), "r"(512));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
   }
   fence_before();
-  __syncthreads();
+  sync_group<CG>();
   fence_after();
   const uint32_t tmem = tmem_sh;
   const int n = it.tiles;
@@ -213,7 +270,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   // what a softmax thread keeps until the end
   const int x = NQ == 2 ? warp >> 2 : 0;                       // its stream of row blocks
   const int rr = (warp & 3) * 32 + lane;                       // its row of the block
-  const int row = it.rb * ROWS + x * 128 + rr;
+  const int row = (it.rb * CG + (int)rank) * ROWS + x * 128 + rr;
   const int qi = row / p.group, tok = it.r.t0 + qi, head = it.h * p.group + row - qi * p.group;
   const bool real = soft && row < it.rows && tok >= 0 && tok < p.tokens;
   const int pos = it.r.pos0 + qi;
@@ -265,7 +322,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     }
     proxy_fence();
     __syncwarp();
-    if (lane == 0) mbar::arrive(mbar::saddr(&q_full));
+    if (lane == 0) arrive_lead<CG>(mbar::saddr(&q_full));
     const float unscale = std::is_same<T, __nv_bfloat16>::value ? row_unscale[x * 128 + rr] : 1.f;
     // score -> log2 units; not zero, so that a masked -inf stays -inf
     c = fmaxf(p.scale_log2 * unscale * p.cache.scales[it.h], 1.2e-38f);
@@ -348,76 +405,94 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       tmem_st_wait();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar::arrive(mbar::saddr(&p_full[buf]));
+      if (lane == 0) arrive_lead<CG>(mbar::saddr(&p_full[buf]));
     }
     if (n > 0) wait(mbar::saddr(&o_done[x]), (n - 1) & 1, &abort_flag);
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < 12) {
       // ---- converters: thread items are 16-channel groups of a key, the same
-      // places in every tile
-      constexpr int NTHR = C::CONV_WARPS * 32, ITEMS = TK * GP / NTHR;
+      // places in every tile.  Of a pair each CTA converts its half of the second
+      // operand's columns: half the keys of K, half the channels of V.
+      constexpr int NTHR = C::CONV_WARPS * 32, ITEMS = TK * GP / (NTHR * CG);
       const int ct = threadIdx.x - (12 - C::CONV_WARPS) * 32;
-      const int BP = min(p.P, TK);
-      uint32_t from[ITEMS], from_s[ITEMS];
+      struct Places {
+        uint32_t from[ITEMS], from_s[ITEMS], to, flip;
+        int row0;
+      };
+      // KEYS keys, GR groups from group g0 on
+      auto places = [&](auto keys, auto groups, int g0) {
+        constexpr int KEYS = decltype(keys)::value, GR = decltype(groups)::value;
+        // item e's row is row0 + e NTHR / GR (a multiple of 8 apart, or the swizzle below would move)
+        static_assert((NTHR / GR) % 8 == 0 && KEYS * GR == ITEMS * NTHR, "rows of a thread's items differ by whole swizzle groups");
+        const int BP = min(p.P, KEYS);
+        Places q;
 #pragma unroll
-      for (int e = 0; e < ITEMS; ++e) {
-        const int key = (ct + e * NTHR) / GP, grp = (ct + e * NTHR) % GP, in = key & (BP - 1);
-        const uint32_t blk = (uint32_t)(key / BP) * L::v_code(BP);
-        from[e] = blk + in * L::CODE + grp * 8;
-        from_s[e] = blk + L::k_scale(BP) + in * L::SCALE + grp;
-      }
-      // item e's row is row0 + e NTHR / GP (a multiple of 8 apart, or the swizzle below would move)
-      static_assert((NTHR / GP) % 8 == 0, "rows of a thread's items differ by whole swizzle groups");
-      const int row0 = ct / GP, grp = ct % GP;
-      // the halves of 8 lanes write different 16-byte columns: groups 4.. write their second chunk first
-      const uint32_t flip = (grp >> 2) & 1;
-      const uint32_t at0 = (grp >> 2) * (TK * 128) + row0 * 128 + ((((grp & 3) * 2 + flip) ^ (row0 & 7)) << 4);
-      bool bad = false;
+        for (int e = 0; e < ITEMS; ++e) {
+          const int key = (ct + e * NTHR) / GR, grp = (ct + e * NTHR) % GR + g0, in = key & (BP - 1);
+          const uint32_t blk = (uint32_t)(key / BP) * L::v_code(BP);
+          q.from[e] = blk + in * L::CODE + grp * 8;
+          q.from_s[e] = blk + L::k_scale(BP) + in * L::SCALE + grp;
+        }
+        const int grp = ct % GR;
+        q.row0 = ct / GR;
+        // the halves of 8 lanes write different 16-byte columns: groups 4.. write their second chunk first
+        q.flip = (grp >> 2) & 1;
+        q.to = (grp >> 2) * (KEYS * 128) + q.row0 * 128 + ((((grp & 3) * 2 + q.flip) ^ (q.row0 & 7)) << 4);
+        return q;
+      };
+      using std::integral_constant;
+      constexpr int KK = TK / CG, VG = GP / CG, K_STEP = NTHR / GP, V_STEP = NTHR / VG;
+      const Places pk = places(integral_constant<int, KK>{}, integral_constant<int, GP>{}, 0);
+      const Places pv = CG == 1 ? pk : places(integral_constant<int, TK>{}, integral_constant<int, VG>{}, (int)rank * VG);
       int slot = 0;  // slots (and stages) so far: K and V of a tile in turn
-      for (int j = 0; j < n && !bad; ++j) {
-        for (int kv = 0; kv < 2 && !bad; ++kv, ++slot) {
-          if (!wait_warp(mbar::saddr(&kv_empty[slot % kSlots]), ((slot / kSlots) & 1) ^ 1, &abort_flag)) { bad = true; break; }
-          const uint32_t out = s_kv + (slot % kSlots) * C::SLOT + at0;
-          const int rs = slot % kRaw;
-          if (!wait_warp(mbar::saddr(&raw_full[rs]), (slot / kRaw) & 1, &abort_flag)) { bad = true; break; }
-          const uint32_t stage = s_rw + rs * C::RAW;
-          uint2 w[ITEMS];
-          uint32_t sc[ITEMS];
+      auto convert = [&](const Places& q, int step, int key0) {
+        if (!wait_warp(mbar::saddr(&kv_empty[slot % kSlots]), ((slot / kSlots) & 1) ^ 1, &abort_flag)) return false;
+        const uint32_t out = s_kv + (slot % kSlots) * C::SLOT + q.to;
+        const int rs = slot % kRaw;
+        if (!wait_warp(mbar::saddr(&raw_full[rs]), (slot / kRaw) & 1, &abort_flag)) return false;
+        const uint32_t stage = s_rw + rs * C::RAW;
+        uint2 w[ITEMS];
+        uint32_t sc[ITEMS];
+#pragma unroll
+        for (int e = 0; e < ITEMS; ++e) {
+          w[e] = lds_u64(stage + q.from[e]);
+          sc[e] = lds_u8(stage + q.from_s[e]);
+        }
+        if (key0 >= 0) {
+          // V: slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
 #pragma unroll
           for (int e = 0; e < ITEMS; ++e) {
-            w[e] = lds_u64(stage + from[e]);
-            sc[e] = lds_u8(stage + from_s[e]);
-          }
-          if (kv) {
-            // slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
-            const int key0 = (it.tile0 + j) * TK + row0;
-#pragma unroll
-            for (int e = 0; e < ITEMS; ++e) {
-              if (key0 + e * (NTHR / GP) >= it.limit) sc[e] = 0;
-              if ((sc[e] & 0x7F) == 0x7F) { nan_seen = 1; sc[e] = 0; }
+            if (key0 + q.row0 + e * step >= it.limit) sc[e] = 0;
+            if ((sc[e] & 0x7F) == 0x7F) {
+              store_all<CG>(mbar::saddr(const_cast<uint32_t*>(&nan_seen)), 1u);
+              sc[e] = 0;
             }
           }
-#pragma unroll
-          for (int e = 0; e < ITEMS; ++e) {
-            const uint32_t s2 = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(sc[e]), 0, 0x1010);
-            const uint32_t x = flip ? w[e].y : w[e].x, y = flip ? w[e].x : w[e].y;
-            const uint32_t dst = out + e * (NTHR / GP) * 128;
-            sts16(dst, hmul2(e2m1x2_to_f16x2<0>(x), s2), hmul2(e2m1x2_to_f16x2<1>(x), s2),
-                  hmul2(e2m1x2_to_f16x2<2>(x), s2), hmul2(e2m1x2_to_f16x2<3>(x), s2));
-            sts16(dst ^ 16, hmul2(e2m1x2_to_f16x2<0>(y), s2), hmul2(e2m1x2_to_f16x2<1>(y), s2),
-                  hmul2(e2m1x2_to_f16x2<2>(y), s2), hmul2(e2m1x2_to_f16x2<3>(y), s2));
-          }
-          __syncwarp();
-          if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));
-          proxy_fence();
-          __syncwarp();
-          if (lane == 0) mbar::arrive(mbar::saddr(&kv_full[slot % kSlots]));
         }
-      }
+#pragma unroll
+        for (int e = 0; e < ITEMS; ++e) {
+          const uint32_t s2 = __byte_perm(fp8x2_to_f16x2<CEK_E4M3>(sc[e]), 0, 0x1010);
+          const uint32_t x = q.flip ? w[e].y : w[e].x, y = q.flip ? w[e].x : w[e].y;
+          const uint32_t dst = out + e * step * 128;
+          sts16(dst, hmul2(e2m1x2_to_f16x2<0>(x), s2), hmul2(e2m1x2_to_f16x2<1>(x), s2),
+                hmul2(e2m1x2_to_f16x2<2>(x), s2), hmul2(e2m1x2_to_f16x2<3>(x), s2));
+          sts16(dst ^ 16, hmul2(e2m1x2_to_f16x2<0>(y), s2), hmul2(e2m1x2_to_f16x2<1>(y), s2),
+                hmul2(e2m1x2_to_f16x2<2>(y), s2), hmul2(e2m1x2_to_f16x2<3>(y), s2));
+        }
+        __syncwarp();
+        if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) arrive_lead<CG>(mbar::saddr(&kv_full[slot % kSlots]));
+        ++slot;
+        return true;
+      };
+      for (int j = 0; j < n; ++j)
+        if (!convert(pk, K_STEP, -1) || !convert(pv, V_STEP, (it.tile0 + j) * TK)) break;
     } else if (warp == 12) {
-      // ---- matrix instructions
-      if (n > 0) {
+      // ---- matrix instructions, of a pair by its first CTA
+      if (n > 0 && rank == 0) {
         bool ok = wait_warp(mbar::saddr(&q_full), 0, &abort_flag);
         auto qk = [&](int j, int st) {  // S = Q K^T into the stream's (tile's) buffer
           const uint32_t d = tmem + (NQ == 2 ? st : j & 1) * 128;
@@ -425,9 +500,9 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              mma_ss(d, desc(a + (k >> 2) * (128 * 128) + (k & 3) * 32, 16), desc(b + (k >> 2) * (TK * 128) + (k & 3) * 32, 16),
+              mma_ss<CG>(d, desc(a + (k >> 2) * (128 * 128) + (k & 3) * 32, 16), desc(b + (k >> 2) * (TK / CG * 128) + (k & 3) * 32, 16),
                      C::IDESC_QK, k > 0);
-            commit(mbar::saddr(&s_full[NQ == 2 ? st : j & 1]));
+            commit<CG>(mbar::saddr(&s_full[NQ == 2 ? st : j & 1]));
           }
           __syncwarp();
         };
@@ -437,13 +512,13 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < TK / 16; ++k)
-              mma_ts(d, a + k * 8, desc(b + k * 2048, TK * 128), C::IDESC_PV, j > 0 || k > 0);
-            commit(mbar::saddr(&o_done[st]));
+              mma_ts<CG>(d, a + k * 8, desc(b + k * 2048, TK * 128), C::IDESC_PV, j > 0 || k > 0);
+            commit<CG>(mbar::saddr(&o_done[st]));
           }
           __syncwarp();
         };
         auto release = [&](int i) {  // slot i once all products issued so far are done
-          if (elect()) commit(mbar::saddr(&kv_empty[i % kSlots]));
+          if (elect()) commit<CG>(mbar::saddr(&kv_empty[i % kSlots]));
           __syncwarp();
         };
         auto kv_ready = [&](int i) { return wait_warp(mbar::saddr(&kv_full[i % kSlots]), (i / kSlots) & 1, &abort_flag); };
@@ -487,10 +562,10 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
             release(2 * j + 1);
           }
         }
-        if (elect()) commit(mbar::saddr(&drain));  // nothing of ours still runs when tensor memory is freed
+        if (elect()) commit<CG>(mbar::saddr(&drain));  // nothing of ours still runs when tensor memory is freed
         __syncwarp();
-        wait(mbar::saddr(&drain), 0, &abort_flag);
       }
+      if (n > 0) wait(mbar::saddr(&drain), 0, &abort_flag);
     } else if (warp == 13) {
       // ---- pages
       Feeder<D, TK> feed;
@@ -501,14 +576,16 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         if (!wait_warp(mbar::saddr(&raw_empty[i % kRaw]), ((i / kRaw) & 1) ^ 1, &abort_flag)) break;
         const int key0 = (it.tile0 + (i >> 1)) * TK;
         if ((i & 1) == 0) feed.look(p, key0, lane);
-        feed.ask_part(p, s_rw + (i % kRaw) * C::RAW, mbar::saddr(&raw_full[i % kRaw]), lane, key0, i & 1);
+        const uint32_t dst = s_rw + (i % kRaw) * C::RAW, bar = mbar::saddr(&raw_full[i % kRaw]);
+        if ((i & 1) == 0) feed.template ask_part<TK / CG>(p, dst, bar, lane, key0 + (int)rank * (TK / CG), 0);
+        else feed.template ask_part<TK>(p, dst, bar, lane, key0, 1);
       }
       for (int a = i > kRaw ? i - kRaw : 0; a < i; ++a)  // no copy of ours is still landing
         wait(mbar::saddr(&raw_full[a % kRaw]), (a / kRaw) & 1, &abort_flag);
     }
   }
 
-  __syncthreads();
+  sync_group<CG>();
   if (soft) {
     // ---- the row's output
     fence_after();
@@ -559,9 +636,12 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     }
     fence_before();
   }
-  __syncthreads();
+  sync_group<CG>();
   fence_after();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  if (warp == 12) {
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
 }
 
 // Joins the splits of a row: four warps a row, each every fourth split, then the
@@ -569,7 +649,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
 template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(128)
 attn_prefill_join_kernel(const AttnParams p, int row_blocks, int splits) {
-  using C = Cfg<D, NQ>;
+  using C = Cfg<D, NQ, 1>;
   constexpr int ROWS = C::ROWS, E = D / 32, SIZE = ROWS * (D + 2);
   __shared__ float red[4][D], red_l[4];
   pdl_launch_dependents();
@@ -616,13 +696,14 @@ attn_prefill_join_kernel(const AttnParams p, int row_blocks, int splits) {
 }
 
 struct Plan {
-  int nq, row_blocks, splits;
+  int nq, cg, row_blocks, splits;
   int64_t items, partial_bytes;
 };
 inline Plan plan_of(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
   Plan r;
   const int64_t rows = max_q * group;
   r.nq = d == 256 || rows <= 128 ? 1 : 2;
+  r.cg = 1;
   r.row_blocks = (int)((rows + 128 * r.nq - 1) / (128 * r.nq));
   r.items = requests * heads * r.row_blocks;
   // too few row blocks for the SMs: split their keys, at least four tiles a piece
@@ -631,26 +712,52 @@ inline Plan plan_of(int64_t d, int64_t requests, int64_t heads, int64_t group, i
   if (r.items < cek_host::sm_count() && tiles >= 8)
     r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cek_host::sm_count() / r.items, tiles / 4));
   r.partial_bytes = r.splits > 1 ? r.items * r.splits * 128 * r.nq * (d + 2) * (int64_t)sizeof(float) : 0;
+  // enough work for all SMs in pairs
+  if (d == 128 && r.nq == 2 && r.splits == 1 && r.items >= 2 * cek_host::sm_count()) {
+    r.cg = 2;
+    r.row_blocks = (int)((rows + 511) / 512);
+    r.items = requests * heads * r.row_blocks;
+  }
   return r;
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, int CG>
 int launch(const AttnParams& p, const Plan& r, cudaStream_t st) {
+  using C = Cfg<D, NQ, CG>;
   static cek_host::DeviceSlots attr;
-  if (!cek_host::ensure_smem_attr(attr, attn_prefill_kernel<T, D, NQ>, Cfg<D, NQ>::SMEM)) return CEK_ERR_LAUNCH;
-  const int64_t blocks = r.items * r.splits;
+  if (!cek_host::ensure_smem_attr(attr, attn_prefill_kernel<T, D, NQ, CG>, C::SMEM)) return CEK_ERR_LAUNCH;
+  const int64_t blocks = r.items * r.splits * CG;
   if (blocks > INT32_MAX) return CEK_ERR_INVALID_ARG;
-  int s = cek_host::launch_pdl(attn_prefill_kernel<T, D, NQ>, dim3((unsigned)blocks), dim3(kThreads), Cfg<D, NQ>::SMEM, st,
-                               p, r.row_blocks, r.splits);
-  if (s != CEK_OK || r.splits == 1) return s;
-  const dim3 grid((unsigned)(p.max_q * p.group), (unsigned)p.cache.heads, (unsigned)p.requests);
-  return cek_host::launch_pdl(attn_prefill_join_kernel<T, D, NQ>, grid, dim3(128), 0, st, p, r.row_blocks, r.splits);
+  if constexpr (CG == 2) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute a[2];
+    a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a[0].val.programmaticStreamSerializationAllowed = cek_host::pdl_enabled() ? 1 : 0;
+    a[1].id = cudaLaunchAttributeClusterDimension;
+    a[1].val.clusterDim.x = 2;
+    a[1].val.clusterDim.y = a[1].val.clusterDim.z = 1;
+    cfg.attrs = a;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, attn_prefill_kernel<T, D, NQ, CG>, p, r.row_blocks, r.splits) == cudaSuccess ? CEK_OK
+                                                                                                              : CEK_ERR_LAUNCH;
+  } else {
+    int s = cek_host::launch_pdl(attn_prefill_kernel<T, D, NQ, CG>, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, p,
+                                 r.row_blocks, r.splits);
+    if (s != CEK_OK || r.splits == 1) return s;
+    const dim3 grid((unsigned)(p.max_q * p.group), (unsigned)p.cache.heads, (unsigned)p.requests);
+    return cek_host::launch_pdl(attn_prefill_join_kernel<T, D, NQ>, grid, dim3(128), 0, st, p, r.row_blocks, r.splits);
+  }
 }
 template <typename T>
 int launch_t(int64_t d, const AttnParams& p, const Plan& r, cudaStream_t st) {
-  if (d == 64) return r.nq == 1 ? launch<T, 64, 1>(p, r, st) : launch<T, 64, 2>(p, r, st);
-  if (d == 128) return r.nq == 1 ? launch<T, 128, 1>(p, r, st) : launch<T, 128, 2>(p, r, st);
-  return launch<T, 256, 1>(p, r, st);
+  if (d == 64) return r.nq == 1 ? launch<T, 64, 1, 1>(p, r, st) : launch<T, 64, 2, 1>(p, r, st);
+  if (d == 256) return launch<T, 256, 1, 1>(p, r, st);
+  if (r.nq == 1) return launch<T, 128, 1, 1>(p, r, st);
+  return r.cg == 1 ? launch<T, 128, 2, 1>(p, r, st) : launch<T, 128, 2, 2>(p, r, st);
 }
 }  // namespace pf
 

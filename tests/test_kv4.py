@@ -585,3 +585,55 @@ def test_attention_no_wait_gave_up(cuda_device):
     count = ctypes.c_uint64(1)
     cabi.call("cek_kv4_timeouts", ctypes.byref(count))
     assert count.value == 0
+
+
+# ---- many rows: every SM busy, CTAs in pairs -----------------------------------------
+
+def attention_by_matrices(dev, c, window):
+    """oracle attention as float64 matrix products on the GPU, for prompts that the row loop would take minutes for."""
+    hq, d = c["q"].shape[1:]
+    hkv = c["cache"].shape[1]
+    out = torch.zeros(c["q"].shape, dtype=torch.float64, device=dev)
+    vmax = torch.zeros(c["q"].shape[:2], dtype=torch.float64, device=dev)
+    for i, n in enumerate(c["seq"].tolist()):
+        a, b = c["start"][i].item(), c["start"][i + 1].item()
+        keys = torch.arange(n)
+        slots = (c["table"][i].long()[keys // c["page"]] * c["page"] + keys % c["page"]).numpy()
+        k, v = (torch.from_numpy(K.decode(c["cache"], c["page"], d, slots, part, c["scales"])).to(dev) for part in (0, 1))
+        pos, keys = (n - (b - a) + torch.arange(b - a, device=dev))[:, None], keys.to(dev)[None]
+        seen = (keys <= pos) & ((keys > pos - window) if window else True)
+        for h in range(hq):
+            s = c["q"][a:b, h].to(dev).double() @ k[:, h * hkv // hq].T * c["scale"]
+            out[a:b, h] = torch.softmax(s.masked_fill(~seen, float("-inf")), -1) @ v[:, h * hkv // hq]
+            top = v[:, h * hkv // hq].abs().amax(-1)
+            vmax[a:b, h] = torch.where(seen, top, 0.0).amax(-1)
+    return out.cpu(), vmax.cpu()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("lens,hq,hkv,dt,window", [([(1201, 1201), (1100, 1333)], 32, 4, "f16", 0),
+                                                   ([(1201, 1300), (1100, 1100)], 32, 4, "bf16", 300),
+                                                   ([(700, 900), (513, 513), (640, 640)], 40, 40, "f16", 0),
+                                                   ([(1500, 1500)], 56, 8, "bf16", 0)])
+def test_attention_many_rows(ext, cuda_device, lens, hq, hkv, dt, window, page):
+    c = attention_case(lens, hq, hkv, 128, page, DT[dt])
+    got = run_attention(ext, cuda_device, c, window).cpu()
+    ref, vmax = attention_by_matrices(cuda_device, c, window)
+    assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
+    assert torch.equal(got, run_attention(ext, cuda_device, c, window).cpu())
+
+
+@pytest.mark.gpu
+def test_attention_many_rows_nan_stays_behind(ext, cuda_device):
+    """A NaN value scale in each half of the channels, seen by the last rows of one head alone."""
+    n, page = 1300, 16
+    c = attention_case([(1201, n), (1100, 1100)], 32, 4, 128, page, torch.float16)
+    ref = run_attention(ext, cuda_device, c).cpu()
+    off = K.offsets(page, 128)
+    nan = torch.zeros_like(ref, dtype=torch.bool)
+    for key, group in ((n - 1, 1), (n - 7, 6)):
+        c["cache"][c["table"][0, key // page].item(), 1, off[3] + (key % page) * 8 + group] = 0x7F
+        nan[1201 - (n - key):1201, 8:16, 16 * group:16 * group + 16] = True
+    got = run_attention(ext, cuda_device, c).cpu()
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], ref[~nan])
