@@ -45,10 +45,12 @@ constexpr int kThreads = 512;
 constexpr uint32_t kPolls = 1u << 24;
 constexpr int kSmem = 226 * 1024;  // dynamic shared memory of a CTA at most
 
-// CG CTAs share their K and V (a cluster; CG = 2 for D = 128, NQ = 2).
+// CG CTAs share their K and V (a cluster).
 template <int D, int NQ, int CG>
 struct Cfg {
-  static constexpr int TK = D == 256 ? 64 : 128;
+  // 128 keys a tile: products of 64 columns take the matrix unit as long as ones of 128.  One
+  // CTA's K and V of 256 channels leave room for 64.
+  static constexpr int TK = D == 256 && CG == 1 ? 64 : 128;
     static constexpr int ROWS = NQ * 128;                   // of a CTA; an item has CG of them
   static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2 / CG, RAW = Layout<D>::v_code(TK);  // a raw stage: a tile's keys or values
   static constexpr int SLOTS = 4;                         // converted K and V tiles
@@ -213,7 +215,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   using C = Cfg<D, NQ, CG>;
   using L = Layout<D>;
   constexpr int TK = C::TK, ROWS = C::ROWS, GP = D / 16;
-  static_assert(CG == 1 || (D == 128 && NQ == 2), "a pair halves V by 64 channels");
+  static_assert(CG == 1 || D >= 128, "a pair halves V by 64 channels at least");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (mbar::saddr(smem_raw) + 1023u) & ~1023u;
   const uint32_t s_q = sbase, s_kv = sbase + C::Q_BYTES, s_rw = s_kv + C::SLOTS * C::SLOT;
@@ -713,9 +715,9 @@ inline Plan plan_of(int64_t d, int64_t requests, int64_t heads, int64_t group, i
     r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cek_host::sm_count() / r.items, tiles / 4));
   r.partial_bytes = r.splits > 1 ? r.items * r.splits * 128 * r.nq * (d + 2) * (int64_t)sizeof(float) : 0;
   // enough work for all SMs in pairs
-  if (d == 128 && r.nq == 2 && r.splits == 1 && r.items >= 2 * cek_host::sm_count()) {
+  if ((d == 256 || (d == 128 && r.nq == 2)) && r.splits == 1 && r.items >= 2 * cek_host::sm_count()) {
     r.cg = 2;
-    r.row_blocks = (int)((rows + 511) / 512);
+    r.row_blocks = (int)((rows + 256 * r.nq - 1) / (256 * r.nq));
     r.items = requests * heads * r.row_blocks;
   }
   return r;
@@ -755,7 +757,7 @@ int launch(const AttnParams& p, const Plan& r, cudaStream_t st) {
 template <typename T>
 int launch_t(int64_t d, const AttnParams& p, const Plan& r, cudaStream_t st) {
   if (d == 64) return r.nq == 1 ? launch<T, 64, 1, 1>(p, r, st) : launch<T, 64, 2, 1>(p, r, st);
-  if (d == 256) return launch<T, 256, 1, 1>(p, r, st);
+  if (d == 256) return r.cg == 1 ? launch<T, 256, 1, 1>(p, r, st) : launch<T, 256, 1, 2>(p, r, st);
   if (r.nq == 1) return launch<T, 128, 1, 1>(p, r, st);
   return r.cg == 1 ? launch<T, 128, 2, 1>(p, r, st) : launch<T, 128, 2, 2>(p, r, st);
 }

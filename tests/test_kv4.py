@@ -612,12 +612,14 @@ def attention_by_matrices(dev, c, window):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("page", [16, 64, 128])
-@pytest.mark.parametrize("lens,hq,hkv,dt,window", [([(1201, 1201), (1100, 1333)], 32, 4, "f16", 0),
-                                                   ([(1201, 1300), (1100, 1100)], 32, 4, "bf16", 300),
-                                                   ([(700, 900), (513, 513), (640, 640)], 40, 40, "f16", 0),
-                                                   ([(1500, 1500)], 56, 8, "bf16", 0)])
-def test_attention_many_rows(ext, cuda_device, lens, hq, hkv, dt, window, page):
-    c = attention_case(lens, hq, hkv, 128, page, DT[dt])
+@pytest.mark.parametrize("lens,hq,hkv,d,dt,window", [([(1201, 1201), (1100, 1333)], 32, 4, 128, "f16", 0),
+                                                     ([(1201, 1300), (1100, 1100)], 32, 4, 128, "bf16", 300),
+                                                     ([(700, 900), (513, 513), (640, 640)], 40, 40, 128, "f16", 0),
+                                                     ([(1500, 1500)], 56, 8, 128, "bf16", 0),
+                                                     ([(1201, 1201), (1100, 1333)], 16, 4, 256, "f16", 0),
+                                                     ([(1300, 1301), (9, 700), (1100, 1100)], 20, 4, 256, "bf16", 77)])
+def test_attention_many_rows(ext, cuda_device, lens, hq, hkv, d, dt, window, page):
+    c = attention_case(lens, hq, hkv, d, page, DT[dt])
     got = run_attention(ext, cuda_device, c, window).cpu()
     ref, vmax = attention_by_matrices(cuda_device, c, window)
     assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
@@ -625,15 +627,16 @@ def test_attention_many_rows(ext, cuda_device, lens, hq, hkv, dt, window, page):
 
 
 @pytest.mark.gpu
-def test_attention_many_rows_nan_stays_behind(ext, cuda_device):
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_many_rows_nan_stays_behind(ext, cuda_device, d):
     """A NaN value scale in each half of the channels, seen by the last rows of one head alone."""
     n, page = 1300, 16
-    c = attention_case([(1201, n), (1100, 1100)], 32, 4, 128, page, torch.float16)
+    c = attention_case([(1201, n), (1100, 1100)], 32, 4, d, page, torch.float16)
     ref = run_attention(ext, cuda_device, c).cpu()
-    off = K.offsets(page, 128)
+    off = K.offsets(page, d)
     nan = torch.zeros_like(ref, dtype=torch.bool)
-    for key, group in ((n - 1, 1), (n - 7, 6)):
-        c["cache"][c["table"][0, key // page].item(), 1, off[3] + (key % page) * 8 + group] = 0x7F
+    for key, group in ((n - 1, 1), (n - 7, d // 16 - 2)):
+        c["cache"][c["table"][0, key // page].item(), 1, off[3] + (key % page) * (d // 16) + group] = 0x7F
         nan[1201 - (n - key):1201, 8:16, 16 * group:16 * group + 16] = True
     got = run_attention(ext, cuda_device, c).cpu()
     assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], ref[~nan])
