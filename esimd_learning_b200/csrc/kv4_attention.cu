@@ -759,7 +759,12 @@ attn_join_kernel(const AttnParams p, int ctas) {
 namespace {
 using namespace cek::kv4;
 
-constexpr int64_t kDecodeRows = 16;  // rows of a kv head that the decode kernel takes
+// Rows of a kv head that the decode kernel takes.  At 17 to 32 rows (two passes of
+// 16) it beats the tensor-core kernel for narrow heads: 16 requests of 5 rows on
+// 16/4 heads of 64, 4000 keys, 24.6 us against 28.6; one of 4 tokens on 64/8 heads
+// of 128, 500 keys, 10.7 against 12.8.  At 256 channels two n8 blocks of rows do
+// not fit its registers: 16 rows on 500 keys 21.5 us against 16.4.
+inline int64_t decode_rows(int64_t d) { return d == 256 ? 8 : 32; }
 
 struct DecodePlan {
   int nt, ctas;
@@ -790,8 +795,9 @@ DecodePlan plan_decode_dn(int64_t requests, int64_t heads, int64_t group, int64_
 }
 template <int D>
 DecodePlan plan_decode_d(int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
-  return max_q * group <= 8 ? plan_decode_dn<D, 1>(requests, heads, group, max_q, max_seq)
-                            : plan_decode_dn<D, 2>(requests, heads, group, max_q, max_seq);
+  if constexpr (D < 256)
+    if (max_q * group > 8) return plan_decode_dn<D, 2>(requests, heads, group, max_q, max_seq);
+  return plan_decode_dn<D, 1>(requests, heads, group, max_q, max_seq);
 }
 DecodePlan plan_decode(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq) {
   return d == 64    ? plan_decode_d<64>(requests, heads, group, max_q, max_seq)
@@ -813,7 +819,7 @@ template <typename T>
 int launch_decode_t(int64_t dim, const AttnParams& p, const DecodePlan& d, cudaStream_t st) {
   if (dim == 64) return d.nt == 1 ? launch_decode<T, 64, 1>(p, d, st) : launch_decode<T, 64, 2>(p, d, st);
   if (dim == 128) return d.nt == 1 ? launch_decode<T, 128, 1>(p, d, st) : launch_decode<T, 128, 2>(p, d, st);
-  return d.nt == 1 ? launch_decode<T, 256, 1>(p, d, st) : launch_decode<T, 256, 2>(p, d, st);
+  return launch_decode<T, 256, 1>(p, d, st);
 }
 }  // namespace
 
@@ -824,7 +830,7 @@ extern "C" int64_t cek_kv4_attention_workspace_bytes(int64_t requests, int64_t t
       max_seq_len <= 0 || !cek_host::kv4_head_dim(head_dim))
     return 0;
   const int64_t group = q_heads / kv_heads, max_q = std::min(max_query_len, tokens);
-  if (max_q * group <= kDecodeRows)
+  if (max_q * group <= decode_rows(head_dim))
     return plan_decode(head_dim, requests, kv_heads, group, max_q, max_seq_len).partial_bytes;
   return cek::kv4::prefill_workspace(head_dim, requests, kv_heads, group, max_q, max_seq_len);
 }
@@ -874,7 +880,7 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
   p.key_limit = (int)(table_width * cache->page_size);
   p.window = (int)window;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
-  if (p.max_q * p.group <= kDecodeRows) {
+  if (p.max_q * p.group <= decode_rows(cache->head_dim)) {
     const DecodePlan d = plan_decode(cache->head_dim, requests, cache->kv_heads, p.group, p.max_q, max_seq_len);
     if (workspace_bytes < d.partial_bytes || (d.partial_bytes > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
     if (d.partial_bytes > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
