@@ -449,8 +449,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       const Places pv = CG == 1 ? pk : places(integral_constant<int, TK>{}, integral_constant<int, VG>{}, (int)rank * VG);
       int slot = 0;  // slots (and stages) so far: K and V of a tile in turn
       auto convert = [&](const Places& q, int step, int key0) {
-        if (!wait_warp(mbar::saddr(&kv_empty[slot % kSlots]), ((slot / kSlots) & 1) ^ 1, &abort_flag)) return false;
-        const uint32_t out = s_kv + (slot % kSlots) * C::SLOT + q.to;
         const int rs = slot % kRaw;
         if (!wait_warp(mbar::saddr(&raw_full[rs]), (slot / kRaw) & 1, &abort_flag)) return false;
         const uint32_t stage = s_rw + rs * C::RAW;
@@ -461,6 +459,10 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           w[e] = lds_u64(stage + q.from[e]);
           sc[e] = lds_u8(stage + q.from_s[e]);
         }
+        __syncwarp();
+        if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));  // the stage is in registers
+        if (!wait_warp(mbar::saddr(&kv_empty[slot % kSlots]), ((slot / kSlots) & 1) ^ 1, &abort_flag)) return false;
+        const uint32_t out = s_kv + (slot % kSlots) * C::SLOT + q.to;
         if (key0 >= 0) {
           // V: slots that no row sees count as zero, and so does a NaN scale (put in at the end): 0 * NaN
 #pragma unroll
@@ -482,8 +484,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           sts16(dst ^ 16, hmul2(e2m1x2_to_f16x2<0>(y), s2), hmul2(e2m1x2_to_f16x2<1>(y), s2),
                 hmul2(e2m1x2_to_f16x2<2>(y), s2), hmul2(e2m1x2_to_f16x2<3>(y), s2));
         }
-        __syncwarp();
-        if (lane == 0) mbar::arrive(mbar::saddr(&raw_empty[rs]));
         proxy_fence();
         __syncwarp();
         if (lane == 0) arrive_lead<CG>(mbar::saddr(&kv_full[slot % kSlots]));
