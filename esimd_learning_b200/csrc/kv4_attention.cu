@@ -389,6 +389,7 @@ attn_decode_kernel(const AttnParams p) {
       bool moved = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        float bias2[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           if (!inside) {
@@ -410,17 +411,25 @@ attn_decode_kernel(const AttnParams p) {
           alpha[nt][j] = now == m[nt][j] ? 1.f : ex2((m[nt][j] - now) * f[nt][j]);
           moved |= now != m[nt][j];
           m[nt][j] = now;
-          float sum = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int rr = 0; rr < 2; ++rr) {
-              float& v = sc[mt][nt][2 * rr + j];
-              v = ex2(__fmaf_rn(v, f[nt][j], bias));
-              sum += v;
-            }
-          l[nt][j] = l[nt][j] * alpha[nt][j] + sum;
+          bias2[j] = bias;
         }
+        // two columns an instruction
+        const uint64_t ff = f32x2(f[nt][0], f[nt][1]), bb = f32x2(bias2[0], bias2[1]);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int rr = 0; rr < 2; ++rr) {
+            float &a = sc[mt][nt][2 * rr], &b = sc[mt][nt][2 * rr + 1];
+            unpack_f32x2(fma_f32x2(f32x2(a, b), ff, bb), a, b);
+            a = ex2(a);
+            b = ex2(b);
+            sum = add_f32x2(sum, f32x2(a, b));
+          }
+        float sa, sb2;
+        unpack_f32x2(sum, sa, sb2);
+        l[nt][0] = l[nt][0] * alpha[nt][0] + sa;
+        l[nt][1] = l[nt][1] * alpha[nt][1] + sb2;
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -455,36 +464,32 @@ attn_decode_kernel(const AttnParams p) {
           pf[nt][0] = movmatrix_t(pack2<__half>(sc[mt][nt][0], sc[mt][nt][1]));
           pf[nt][1] = movmatrix_t(pack2<__half>(sc[mt][nt][2], sc[mt][nt][3]));
         }
-        uint32_t w[4][VW], vs[2][VG];
-        uint32_t raw[VG];
-#pragma unroll
-        for (int j = 0; j < VG; ++j) raw[j] = 0;
+        uint32_t w[4][VW], vs[2][VG], sb8[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t code = sb + v_code[mt] + 4 * q * L::CODE, sca = sb + v_sca[mt] + 4 * q * L::SCALE;
           if constexpr (D == 64) {
             w[q][0] = lds_u32(code);
-            raw[0] |= lds_u8(sca) << (8 * q);
+            sb8[q] = lds_u8(sca);
           } else if constexpr (D == 128) {
             const uint2 v = lds_u64(code);
             w[q][0] = v.x;
             w[q][1] = v.y;
-            raw[0] |= lds_u8(sca) << (8 * q);
+            sb8[q] = lds_u8(sca);
           } else {
             const uint4 v = mbar::lds16(code);
             w[q][0] = v.x;
             w[q][1] = v.y;
             w[q][2] = v.z;
             w[q][3] = v.w;
-            const uint32_t two = lds_u16(sca);
-            raw[0] |= (two & 0xFFu) << (8 * q);
-            raw[1] |= (two >> 8) << (8 * q);
+            sb8[q] = lds_u16(sca);
           }
         }
+        // scales of keys t, t + 4 and of t + 8, t + 12
 #pragma unroll
         for (int j = 0; j < VG; ++j) {
-          vs[0][j] = scales_no_nan(raw[j]);
-          vs[1][j] = scales_no_nan(raw[j] >> 16);
+          vs[0][j] = scales_no_nan(__byte_perm(sb8[0], sb8[1], j ? 0x0051 : 0x0040));
+          vs[1][j] = scales_no_nan(__byte_perm(sb8[2], sb8[3], j ? 0x0051 : 0x0040));
         }
 #pragma unroll
         for (int u = 0; u < VW; ++u) {
