@@ -837,7 +837,7 @@ extern "C" int64_t cek_kv4_attention_workspace_bytes(int64_t requests, int64_t t
   const int64_t group = q_heads / kv_heads, max_q = std::min(max_query_len, tokens);
   if (max_q * group <= decode_rows(head_dim))
     return plan_decode(head_dim, requests, kv_heads, group, max_q, max_seq_len).partial_bytes;
-  return cek::kv4::prefill_workspace(head_dim, requests, kv_heads, group, max_q, max_seq_len);
+  return cek::kv4::prefill_workspace(head_dim, requests, tokens, kv_heads, group, max_q, max_seq_len);
 }
 
 extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, const int32_t* block_table,
@@ -902,7 +902,8 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
     }
     return rc;
   }
-  const int64_t need = cek::kv4::prefill_workspace(cache->head_dim, requests, cache->kv_heads, p.group, p.max_q, max_seq_len);
+  const int64_t need = cek::kv4::prefill_workspace(cache->head_dim, requests, tokens, cache->kv_heads, p.group,
+                                                        p.max_q, max_seq_len);
   if (workspace_bytes < need || (need > 0 && !workspace)) return CEK_ERR_INVALID_ARG;
   if (need > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
   p.partial = static_cast<float*>(workspace);

@@ -23,7 +23,8 @@ struct AttnParams {
 };
 
 // kv4_prefill.cu
-int64_t prefill_workspace(int64_t d, int64_t requests, int64_t heads, int64_t group, int64_t max_q, int64_t max_seq);
+int64_t prefill_workspace(int64_t d, int64_t requests, int64_t tokens, int64_t heads, int64_t group, int64_t max_q,
+                          int64_t max_seq);
 int prefill_launch(int dtype, int64_t d, const AttnParams& p, int64_t max_seq, cudaStream_t st);
 bool prefill_timeouts(unsigned long long* count);
 

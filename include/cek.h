@@ -409,6 +409,9 @@ CEK_API int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, voi
  * host (a longer request is read as if cut there: its rows past the bound are
  * not written, its keys past it not read); seq_lens are also cut to
  * table_width * P.  Page numbers outside the cache are clamped into it.
+ * A step that mixes single tokens with prompts is right in one call, but the
+ * prompts' kernel then takes all of it: two calls with slices of the request
+ * arrays (query_start holds rows of the whole query) give each its own.
  * workspace: cek_kv4_attention_workspace_bytes() bytes, 16-byte aligned,
  * contents ignored; may be null where that is 0.  One call at a time per
  * workspace.  Deterministic: no atomics order a sum. */

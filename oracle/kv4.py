@@ -37,7 +37,7 @@ def nearest_even(x: np.ndarray, grid: np.ndarray) -> np.ndarray:
 
 def quantize(x: torch.Tensor, g: torch.Tensor):
     """x [T, H, D] (16-bit), g [H] fp32 -> (packed codes uint8 [T, H, D/2], scale bytes uint8 [T, H, D/16])."""
-    v = x.float().numpy().reshape(x.shape[0], x.shape[1], -1, 16)
+    v = x.float().numpy().reshape(x.shape[0], x.shape[1], x.shape[2] // 16, 16)
     gg = g.float().numpy()[None, :, None]
     with np.errstate(all="ignore"):
         a = np.abs(v).max(-1)  # NaN stays NaN

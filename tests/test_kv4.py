@@ -164,7 +164,7 @@ def run_plan(ext, dev, q, c, table, pool, count, page, tokens, alias=False):
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,qmax,cmax,page", [(1, 1, 0, 16), (1, 1, 15, 16), (1, 40, 16, 16), (5, 1, 100, 32),
                                               (33, 9, 300, 64), (1023, 3, 50, 16), (1025, 7, 200, 128), (4096, 5, 64, 16),
-                                              (7, 3000, 10, 16), (3, 9, 20, 1), (6, 11, 40, 12)])
+                                              (7, 3000, 10, 16), (9, 9000, 50, 32), (3, 9, 20, 1), (6, 11, 40, 12)])
 @pytest.mark.parametrize("room", ["enough", "short", "none"])
 @pytest.mark.parametrize("alias", [False, True])
 def test_plan(ext, cuda_device, B, qmax, cmax, page, room, alias):
@@ -597,6 +597,8 @@ def attention_by_matrices(dev, c, window):
     vmax = torch.zeros(c["q"].shape[:2], dtype=torch.float64, device=dev)
     for i, n in enumerate(c["seq"].tolist()):
         a, b = c["start"][i].item(), c["start"][i + 1].item()
+        if a == b:
+            continue
         keys = torch.arange(n)
         slots = (c["table"][i].long()[keys // c["page"]] * c["page"] + keys % c["page"]).numpy()
         k, v = (torch.from_numpy(K.decode(c["cache"], c["page"], d, slots, part, c["scales"])).to(dev) for part in (0, 1))
@@ -624,6 +626,37 @@ def test_attention_many_rows(ext, cuda_device, lens, hq, hkv, d, dt, window, pag
     ref, vmax = attention_by_matrices(cuda_device, c, window)
     assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
     assert torch.equal(got, run_attention(ext, cuda_device, c, window).cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d", [(8, 1, 128), (32, 8, 128), (4, 1, 64), (16, 8, 256)])
+def test_attention_one_prompt_among_single_tokens(ext, cuda_device, hq, hkv, d):
+    """One long request decides the kernel; 600 short ones (some of nothing) around it."""
+    gen = torch.Generator().manual_seed(7)
+    short = torch.randint(0, 40, (600,), generator=gen).tolist()
+    lens = [(1 if n else 0, n) for n in short]
+    lens[311] = (777, 790)
+    lens[599] = (5, 33)
+    c = attention_case(lens, hq, hkv, d, 16, torch.bfloat16)
+    got = run_attention(ext, cuda_device, c).cpu()
+    ref, vmax = attention_by_matrices(cuda_device, c, 0)
+    assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
+    # the same in two calls: slices of the request arrays
+    out = torch.full_like(got, 77.0, device=cuda_device)
+    for part, longest in ((slice(0, 311), 1), (slice(311, 312), 777), (slice(312, 600), 5)):
+        run_attention(ext, cuda_device, dict(c, table=c["table"][part], seq=c["seq"][part],
+                                             start=c["start"][part.start:part.stop + 1]), max_q=longest, out=out)
+    assert ((out.cpu().double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q", [1, 100])
+def test_attention_of_no_keys(ext, cuda_device, q):
+    c = attention_case([(q, 0), (q, -4)], 4, 2, 64, 16, torch.float16)
+    assert not run_attention(ext, cuda_device, c, max_seq=0).any()
+    assert not run_attention(ext, cuda_device, c, max_seq=500).any()
+    c["table"] = c["table"][:, :0]
+    assert not run_attention(ext, cuda_device, c, max_seq=500).any()
 
 
 @pytest.mark.gpu
