@@ -194,14 +194,15 @@ struct Item {
 // request by request.
 template <int TK, int ROWS, int CG>
 CEK_DEVICE bool item_of(const AttnParams& p, int row_blocks, int splits, Item& it) {
-  int64_t id = blockIdx.x / CG;
-  it.split = (int)(id % splits);
-  id /= splits;
-  it.h = (int)(id % p.cache.heads);
-  id /= p.cache.heads;
+  uint32_t id = blockIdx.x / CG;
+  const uint32_t sp = id / (uint32_t)splits;
+  it.split = (int)(id - sp * (uint32_t)splits);
+  id = sp / (uint32_t)p.cache.heads;
+  it.h = (int)(sp - id * (uint32_t)p.cache.heads);
   if (row_blocks > 0) {
-    it.b = (int)(id % p.requests);
-    it.rb = row_blocks - 1 - (int)(id / p.requests);
+    const uint32_t up = id / (uint32_t)p.requests;
+    it.b = (int)(id - up * (uint32_t)p.requests);
+    it.rb = row_blocks - 1 - (int)up;
   } else {
     __shared__ int sums[kThreads / 32], found[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -272,10 +273,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
 
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRaw; ++i) {
-      mbar::init(mbar::saddr(&raw_full[i]), 1);
-      mbar::init(mbar::saddr(&raw_empty[i]), C::CONV_WARPS);
-    }
     for (int i = 0; i < kSlots; ++i) {
       mbar::init(mbar::saddr(&kv_full[i]), CG * C::CONV_WARPS);
       mbar::init(mbar::saddr(&kv_empty[i]), 1);
@@ -295,6 +292,43 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   Item it;
   if (!item_of<TK, CG * ROWS, CG>(p, row_blocks, splits, it)) return;  // the whole group
   const uint32_t rank = CG == 1 ? 0 : cta_rank();
+  const int n = it.tiles;
+  const bool soft = warp < 4 * NQ;
+
+  // what a softmax thread keeps until the end
+  const int x = NQ == 2 ? warp >> 2 : 0;                       // its stream of row blocks
+  const int rr = (warp & 3) * 32 + lane;                       // its row of the block
+  const int row = (it.rb * CG + (int)rank) * ROWS + x * 128 + rr;
+  const int qi = row / p.group, tok = it.r.t0 + qi, head = it.h * p.group + row - qi * p.group;
+  const bool real = soft && row < it.rows && tok >= 0 && tok < p.tokens;
+  const int pos = it.r.pos0 + qi;
+  const int hi = row < it.rows ? min(pos + 1, it.r.end) : 0, lo = p.window > 0 ? pos - p.window + 1 : 0;
+
+  constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row of Q or of the output, rows at a time
+  const int ch = lane % LPR;
+
+  // the first pages are on their way before the group meets
+  Feeder<D, TK> feed;
+  int pages = 0;  // stages asked for
+  auto ask = [&](int i) {
+    const int key0 = (it.tile0 + (i >> 1)) * TK;
+    if ((i & 1) == 0) feed.look(p, key0, lane);
+    const uint32_t dst = s_rw + (i % kRaw) * C::RAW, bar = mbar::saddr(&raw_full[i % kRaw]);
+    if ((i & 1) == 0) feed.template ask_part<TK / CG>(p, dst, bar, lane, key0 + (int)rank * (TK / CG), 0);
+    else feed.template ask_part<TK>(p, dst, bar, lane, key0, 1);
+  };
+  if (warp == 13) {
+    if (lane == 0) {
+      for (int i = 0; i < kRaw; ++i) {
+        mbar::init(mbar::saddr(&raw_full[i]), 1);
+        mbar::init(mbar::saddr(&raw_empty[i]), C::CONV_WARPS);
+      }
+      mbar::fence_init();
+    }
+    __syncwarp();
+    if (n > 0) feed.load(p, it.b, it.h, it.tile0, n, it.limit, lane);
+    for (; pages < min(2 * n, min(2, kRaw)); ++pages) ask(pages);  // one tile: more would hold up the others
+  }
   if (warp == 12) {
     if constexpr (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(mbar::saddr(&tmem_sh)), "r"(512));
@@ -308,17 +342,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   sync_group<CG>();
   fence_after();
   const uint32_t tmem = tmem_sh;
-  const int n = it.tiles;
-  const bool soft = warp < 4 * NQ;
-
-  // what a softmax thread keeps until the end
-  const int x = NQ == 2 ? warp >> 2 : 0;                       // its stream of row blocks
-  const int rr = (warp & 3) * 32 + lane;                       // its row of the block
-  const int row = (it.rb * CG + (int)rank) * ROWS + x * 128 + rr;
-  const int qi = row / p.group, tok = it.r.t0 + qi, head = it.h * p.group + row - qi * p.group;
-  const bool real = soft && row < it.rows && tok >= 0 && tok < p.tokens;
-  const int pos = it.r.pos0 + qi;
-  const int hi = row < it.rows ? min(pos + 1, it.r.end) : 0, lo = p.window > 0 ? pos - p.window + 1 : 0;
   const uint32_t tm_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   float m = -INFINITY, l = 0.f, c = 0.f;
 
@@ -327,10 +350,9 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ---- Q: the warp's 32 rows, whole rows at a time; 16-byte chunk ch of
     // 64-channel block cb goes to ch ^ (row & 7)
-    constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row, rows at a time
-    constexpr int FLY = 32 / RPI < 16 ? 32 / RPI : 16;  // loads in flight
+    constexpr int MOST = NQ == 1 ? 32 : 16, FLY = 32 / RPI < MOST ? 32 / RPI : MOST;  // loads in flight
+    const uint32_t q_rows = s_q + x * (128 * D * 2) + (ch >> 3) * (128 * 128);
     const int64_t own = real ? (int64_t)tok * p.qts + (int64_t)head * p.qhs : -1;
-    const int ch = lane % LPR;
 #pragma unroll
     for (int i0 = 0; i0 < 32; i0 += FLY * RPI) {
       uint4 v[FLY];
@@ -360,8 +382,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
             u[q] = pack2<__half>(f.x * up, f.y * up);
           }
         }
-        sts16(s_q + x * (128 * D * 2) + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[i].x, v[i].y,
-              v[i].z, v[i].w);
+        sts16(q_rows + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[i].x, v[i].y, v[i].z, v[i].w);
       }
     }
     proxy_fence();
@@ -612,17 +633,10 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       if (n > 0) wait(mbar::saddr(&drain), 0, &abort_flag);
     } else if (warp == 13) {
       // ---- pages
-      Feeder<D, TK> feed;
-      const int total = n * 2;
-      if (n > 0) feed.load(p, it.b, it.h, it.tile0, n, it.limit, lane);
-      int i = 0;
-      for (; i < total; ++i) {
+      int i = pages;
+      for (; i < 2 * n; ++i) {
         if (!wait_warp(mbar::saddr(&raw_empty[i % kRaw]), ((i / kRaw) & 1) ^ 1, &abort_flag)) break;
-        const int key0 = (it.tile0 + (i >> 1)) * TK;
-        if ((i & 1) == 0) feed.look(p, key0, lane);
-        const uint32_t dst = s_rw + (i % kRaw) * C::RAW, bar = mbar::saddr(&raw_full[i % kRaw]);
-        if ((i & 1) == 0) feed.template ask_part<TK / CG>(p, dst, bar, lane, key0 + (int)rank * (TK / CG), 0);
-        else feed.template ask_part<TK>(p, dst, bar, lane, key0, 1);
+        ask(i);
       }
       for (int a = i > kRaw ? i - kRaw : 0; a < i; ++a)  // no copy of ours is still landing
         wait(mbar::saddr(&raw_full[a % kRaw]), (a / kRaw) & 1, &abort_flag);
@@ -646,7 +660,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
       }
     }
     const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : vf / l;
-    T* dst = static_cast<T*>(p.out) + (int64_t)(real ? tok : 0) * p.ots + (int64_t)(real ? head : 0) * p.ohs;
     float* part = p.partial + (int64_t)blockIdx.x * (ROWS * (D + 2));
     if (splits > 1 && real) {
       part[x * 128 + rr] = m == -INFINITY ? m : m * c;
@@ -664,18 +677,34 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
         for (int q = 0; q < 32; ++q) o[q] = 0.f;
       }
 #pragma unroll
-      for (int q = 0; q < 32; ++q) {
-        o[q] *= inv;
-        if ((nan_groups >> ((i + q) >> 4)) & 1) o[q] = __int_as_float(0x7fffffff);
+      for (int q = 0; q < 32; ++q) o[q] *= inv;
+      if (nan_groups) {
+#pragma unroll
+        for (int q = 0; q < 32; ++q)
+          if ((nan_groups >> ((i + q) >> 4)) & 1) o[q] = __int_as_float(0x7fffffff);
       }
       if (splits > 1 && real) {
 #pragma unroll
         for (int q = 0; q < 32; q += 4) *reinterpret_cast<float4*>(part + i + q) = make_float4(o[q], o[q + 1], o[q + 2], o[q + 3]);
-      } else if (real) {
+      } else {
+        // by way of Q's place in shared memory: a row a thread would touch 32 lines a store
 #pragma unroll
-        for (int q = 0; q < 32; q += 8)
-          *reinterpret_cast<uint4*>(dst + i + q) = make_uint4(pack2<T>(o[q], o[q + 1]), pack2<T>(o[q + 2], o[q + 3]),
-                                                              pack2<T>(o[q + 4], o[q + 5]), pack2<T>(o[q + 6], o[q + 7]));
+        for (int q = 0; q < 32; q += 8) {
+          const int c16 = (i + q) / 8;
+          sts16(s_q + x * (128 * D * 2) + (c16 >> 3) * (128 * 128) + rr * 128 + (((c16 & 7) ^ (rr & 7)) << 4),
+                pack2<T>(o[q], o[q + 1]), pack2<T>(o[q + 2], o[q + 3]), pack2<T>(o[q + 4], o[q + 5]), pack2<T>(o[q + 6], o[q + 7]));
+        }
+      }
+    }
+    if (splits == 1) {
+      __syncwarp();
+      const int64_t to = real ? (int64_t)tok * p.ots + (int64_t)head * p.ohs : -1;
+#pragma unroll 8
+      for (int i = 0; i < 32; i += RPI) {
+        const int r = i + lane / LPR, rw = (warp & 3) * 32 + r;
+        const int64_t at = __shfl_sync(0xffffffffu, to, r);
+        const uint4 u = mbar::lds16(s_q + x * (128 * D * 2) + (ch >> 3) * (128 * 128) + rw * 128 + (((ch & 7) ^ (rw & 7)) << 4));
+        if (at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + at + ch * 8) = u;
       }
     }
     fence_before();
