@@ -3,24 +3,34 @@
 //
 // A CTA takes NQ x 128 rows (query token x head of the kv head's group) and the
 // tiles of TK keys that any of them sees.  16 warps:
-//  * softmax (one warpgroup per 128 rows, a thread a row): stages its row of Q
-//    in shared memory, then per tile reads S from tensor memory, keeps the
+//  * softmax (one warpgroup per 128 rows, a thread a row): stages Q in shared
+//    memory, then per tile reads S from tensor memory, keeps the
 //    running maximum and sum, and writes P (fp16) over S;
 //  * converters: turn the codes of a page into the fp16 operands, exactly
 //    (kv4.cuh), straight into the 128-byte-swizzled layout that the matrix unit
 //    reads; a ring of slots K(j), V(j), K(j+1), ...
 //  * one warp copies pages (a bulk copy per page, keys and values apart) into a raw
 //    ring, in the order in which the converters free it;
-//  * one thread issues the matrix instructions: S = Q K^T with both operands in
+//  * one warp issues the matrix instructions: S = Q K^T with both operands in
 //    shared memory, O += P V with P in tensor memory and V read with keys as
 //    the strided dimension, so V needs no transpose.
 // With NQ = 2 the two row blocks take turns: while one's S is in softmax the
 // other's products run.  D = 256 fills tensor memory with one O, so NQ = 1 and
 // the tiles take turns instead (S double-buffered).
 //
-// Bounds at D = 128, per 256 rows x 128 keys: 2048 cycles of matrix unit, 2048
-// of exp2 (16 a cycle), ~2200 of shared memory (1536 of operand reads, 512 of
-// converted writes).
+// With work for every SM, D >= 128 runs on pairs of CTAs (CG = 2,
+// cta_group::2): a product has 256 rows, each CTA keeps and reads half of K's
+// rows and of V's channels, and so converts half.  Alone, the first product is
+// bound by its operands (128 bytes a cycle of shared memory, all of it) and
+// takes 920 cycles instead of 512 beside the converters.
+//
+// Per 256 rows x 128 keys at D = 128 a CTA needs 2048 cycles of matrix unit,
+// 2048 of exp2 (16 a cycle) and, in a pair, ~1500 of shared memory.  It takes
+// ~3500: a row block's softmax (2000) and its products (1024) follow each other,
+// and each hand-over costs a few hundred cycles; two row blocks hide a part of it.
+// 8192 tokens of 64/8 heads of 128 from an empty cache: 1105 us, 995 TFLOP/s.  Six
+// ragged chunks of 16/4 heads of 256 with a window of 1024: 164 us, 501 TFLOP/s;
+// there the 5 us in which an item starts and ends are a third of its time.
 //
 // The output is rescaled only when a row's maximum has grown by more than
 // 2^kLazy since the last time: P is at most 2^(kShift + kLazy) = 2^14 then,
@@ -51,8 +61,9 @@ struct Cfg {
   // 128 keys a tile: products of 64 columns take the matrix unit as long as ones of 128.  One
   // CTA's K and V of 256 channels leave room for 64.
   static constexpr int TK = D == 256 && CG == 1 ? 64 : 128;
-    static constexpr int ROWS = NQ * 128;                   // of a CTA; an item has CG of them
-  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2 / CG, RAW = Layout<D>::v_code(TK);  // a raw stage: a tile's keys or values
+  static constexpr int ROWS = NQ * 128;                   // of a CTA; an item has CG of them
+  static constexpr int Q_BYTES = ROWS * D * 2, SLOT = TK * D * 2 / CG;
+  static constexpr int RAW = Layout<D>::v_code(TK);       // a raw stage: a tile's keys or values
   static constexpr int SLOTS = 4;                         // converted K and V tiles
   // raw stages: what is left, 16 at most
   static constexpr int RAW_ROOM = (kSmem - 1024 - Q_BYTES - SLOTS * SLOT) / RAW, RAWS = RAW_ROOM < 16 ? RAW_ROOM : 16;
@@ -369,8 +380,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
           uint32_t mx = __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
                                  __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
           mx = max(mx & 0xFFFFu, mx >> 16);
-#pragma unroll
-          for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          mx = __reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (lane / LPR * LPR), mx);
           const int e = (int)(mx >> 7);
           const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
           const float up = __int_as_float((127 + k) << 23);
