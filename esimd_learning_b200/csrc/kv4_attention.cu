@@ -198,9 +198,12 @@ attn_decode_kernel(const AttnParams p) {
   const Ranges ranges(prefix[p.requests], Ranges::share_of(prefix[p.requests], (int)gridDim.x, p.pad_tiles));
   const int from = ranges.at(blockIdx.x, warp), to = ranges.at(blockIdx.x, warp + 1);
   bool merge = false;  // the CTA is inside one segment
-  if (ranges.at(blockIdx.x, 0) < ranges.total) {
-    const Segment s = segment_at<TK, ROWS>(p, prefix, ranges.at(blockIdx.x, 0));
-    merge = ranges.merged(blockIdx.x, s.first, s.first + s.tiles);
+  Segment cur = {};    // the segment of this warp's next tile, while it is known
+  const int cta0 = ranges.at(blockIdx.x, 0);
+  if (cta0 < ranges.total) {
+    cur = segment_at<TK, ROWS>(p, prefix, cta0);
+    merge = ranges.merged(blockIdx.x, cur.first, cur.first + cur.tiles);
+    if (from < to && from >= cur.first + cur.tiles) cur = segment_at<TK, ROWS>(p, prefix, from);
   }
   const uint32_t ring = mbar::saddr(smem) + warp * C::STAGES * C::STAGE;
   const int BP = min(p.P, TK);              // tokens of a block in the ring
@@ -232,7 +235,7 @@ attn_decode_kernel(const AttnParams p) {
   feed.left = 0;
   auto ask = [&]() {
     if (feed.left == 0) {
-      const Segment s = segment_at<TK, ROWS>(p, prefix, asked);
+      const Segment s = asked < cur.first + cur.tiles ? cur : segment_at<TK, ROWS>(p, prefix, asked);
       feed.load(p, s.b, s.h, s.r.tile0 + asked - s.first, s.first + s.tiles - asked, s.r.end, lane);
     }
     const int st = (asked - from) % C::STAGES;
@@ -245,7 +248,8 @@ attn_decode_kernel(const AttnParams p) {
   int tile = from;
   while (tile < to) {
     // ---- a segment: its rows' queries as the first product's second operand
-    const Segment s = segment_at<TK, ROWS>(p, prefix, tile);
+    if (tile >= cur.first + cur.tiles) cur = segment_at<TK, ROWS>(p, prefix, tile);
+    const Segment s = cur;
     const int rows = s.r.n * p.group;
     uint32_t qf[NT][STEPS][2];
     float f[NT][2];          // score -> log2 units, per column
@@ -606,7 +610,7 @@ attn_decode_kernel(const AttnParams p) {
   if (!merge) return;
 
   // ---- the four warps' pieces of the one segment, in the order of the keys
-  const Segment s = segment_at<TK, ROWS>(p, prefix, ranges.at(blockIdx.x, 0));
+  const Segment s = cur;
   const int rows = s.r.n * p.group;
   const bool whole = ranges.at(blockIdx.x, 0) == s.first && ranges.at(blockIdx.x, kDecodeWarps) == s.first + s.tiles;
   __syncthreads();
