@@ -318,7 +318,22 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row of Q or of the output, rows at a time
   const int ch = lane % LPR;
 
-  // the first pages are on their way before the group meets
+  // Q and the first pages are on their way before the group meets (with plain loads the
+  // barrier would wait for Q).  Q: the warp's 32 rows, whole rows at a time; 16-byte
+  // chunk ch of 64-channel block cb goes to ch ^ (row & 7); rows that are not there are 0.
+  auto q_at = [&](int i) {
+    const int r = (warp & 3) * 32 + i * RPI + lane / LPR;
+    return s_q + x * (128 * D * 2) + (ch >> 3) * (128 * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+  };
+  if (soft) {
+    const int64_t own = real ? (int64_t)tok * p.qts + (int64_t)head * p.qhs : -1;
+#pragma unroll 8
+    for (int i = 0; i < LPR; ++i) {
+      const int64_t at = __shfl_sync(0xffffffffu, own, i * RPI + lane / LPR);
+      const T* src = static_cast<const T*>(p.q) + max(at, (int64_t)0) + ch * 8;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_at(i)), "l"(src), "r"(at >= 0 ? 16 : 0) : "memory");
+    }
+  }
   Feeder<D, TK> feed;
   int pages = 0;  // stages asked for
   auto ask = [&](int i) {
@@ -359,40 +374,23 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   if (soft) {
     if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    // ---- Q: the warp's 32 rows, whole rows at a time; 16-byte chunk ch of
-    // 64-channel block cb goes to ch ^ (row & 7)
-    constexpr int MOST = NQ == 1 ? 32 : 16, FLY = 32 / RPI < MOST ? 32 / RPI : MOST;  // loads in flight
-    const uint32_t q_rows = s_q + x * (128 * D * 2) + (ch >> 3) * (128 * 128);
-    const int64_t own = real ? (int64_t)tok * p.qts + (int64_t)head * p.qhs : -1;
-#pragma unroll
-    for (int i0 = 0; i0 < 32; i0 += FLY * RPI) {
-      uint4 v[FLY];
-#pragma unroll
-      for (int i = 0; i < FLY; ++i) {
-        const int64_t at = __shfl_sync(0xffffffffu, own, i0 + i * RPI + lane / LPR);
-        v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + at + ch * 8) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < FLY; ++i) {
-        const int r = (warp & 3) * 32 + i0 + i * RPI + lane / LPR;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          // as in the decode kernel: a power of two a row, exactly, into fp16's range
-          uint32_t mx = __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
-                                 __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
-          mx = max(mx & 0xFFFFu, mx >> 16);
-          mx = __reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (lane / LPR * LPR), mx);
-          const int e = (int)(mx >> 7);
-          const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
-          const float up = __int_as_float((127 + k) << 23);
-          if (ch == 0) row_unscale[x * 128 + r] = __int_as_float((127 - k) << 23);
-          uint32_t* u = reinterpret_cast<uint32_t*>(&v[i]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float2 f = unpack2<T>(u[q]);
-            u[q] = pack2<__half>(f.x * up, f.y * up);
-          }
-        }
-        sts16(q_rows + r * 128 + (((ch & 7) ^ (r & 7)) << 4), v[i].x, v[i].y, v[i].z, v[i].w);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      // as in the decode kernel: each row by a power of two, exactly, into fp16's range; a lane
+      // converts the chunks that it has copied
+#pragma unroll 8
+      for (int i = 0; i < LPR; ++i) {
+        uint4 v = mbar::lds16(q_at(i));
+        uint32_t mx = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+        mx = max(mx & 0xFFFFu, mx >> 16);
+        mx = __reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (lane / LPR * LPR), mx);
+        const int e = (int)(mx >> 7);
+        const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
+        const float up = __int_as_float((127 + k) << 23);
+        if (ch == 0) row_unscale[x * 128 + (warp & 3) * 32 + i * RPI + lane / LPR] = __int_as_float((127 - k) << 23);
+        const float2 f0 = unpack2<T>(v.x), f1 = unpack2<T>(v.y), f2 = unpack2<T>(v.z), f3 = unpack2<T>(v.w);
+        sts16(q_at(i), pack2<__half>(f0.x * up, f0.y * up), pack2<__half>(f1.x * up, f1.y * up),
+              pack2<__half>(f2.x * up, f2.y * up), pack2<__half>(f3.x * up, f3.y * up));
       }
     }
     proxy_fence();
