@@ -28,9 +28,9 @@
 // 2048 of exp2 (16 a cycle) and, in a pair, ~1500 of shared memory.  It takes
 // ~3500: a row block's softmax (2000) and its products (1024) follow each other,
 // and each hand-over costs a few hundred cycles; two row blocks hide a part of it.
-// 8192 tokens of 64/8 heads of 128 from an empty cache: 1105 us, 995 TFLOP/s.  Six
-// ragged chunks of 16/4 heads of 256 with a window of 1024: 164 us, 501 TFLOP/s;
-// there the 5 us in which an item starts and ends are a third of its time.
+// 8192 tokens of 64/8 heads of 128 from an empty cache: 1078 us, 1020 TFLOP/s.  Six
+// ragged chunks of 16/4 heads of 256 with a window of 1024: 148 us, 553 TFLOP/s;
+// there an item starts for 6 us and ends for 3 of its 27.
 //
 // The output is rescaled only when a row's maximum has grown by more than
 // 2^kLazy since the last time: P is at most 2^(kShift + kLazy) = 2^14 then,
@@ -369,7 +369,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   fence_after();
   const uint32_t tmem = tmem_sh;
   const uint32_t tm_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-  float m = -INFINITY, l = 0.f, c = 0.f;
+  float m = -INFINITY, l = 0.f, c = 0.f, vf = 0.f;
 
   if (soft) {
     if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
@@ -378,24 +378,36 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       // as in the decode kernel: each row by a power of two, exactly, into fp16's range; a lane
       // converts the chunks that it has copied
-#pragma unroll 8
-      for (int i = 0; i < LPR; ++i) {
-        uint4 v = mbar::lds16(q_at(i));
-        uint32_t mx = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-        mx = max(mx & 0xFFFFu, mx >> 16);
-        mx = __reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (lane / LPR * LPR), mx);
-        const int e = (int)(mx >> 7);
-        const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
-        const float up = __int_as_float((127 + k) << 23);
-        if (ch == 0) row_unscale[x * 128 + (warp & 3) * 32 + i * RPI + lane / LPR] = __int_as_float((127 - k) << 23);
-        const float2 f0 = unpack2<T>(v.x), f1 = unpack2<T>(v.y), f2 = unpack2<T>(v.z), f3 = unpack2<T>(v.w);
-        sts16(q_at(i), pack2<__half>(f0.x * up, f0.y * up), pack2<__half>(f1.x * up, f1.y * up),
-              pack2<__half>(f2.x * up, f2.y * up), pack2<__half>(f3.x * up, f3.y * up));
+#pragma unroll 1
+      for (int i0 = 0; i0 < LPR; i0 += 8) {  // eight rows' chains side by side
+        uint4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mbar::lds16(q_at(i0 + i));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t mx = __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu),
+                                 __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu));
+          mx = max(mx & 0xFFFFu, mx >> 16);
+          mx = __reduce_max_sync(LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1) << (lane / LPR * LPR), mx);
+          const int e = (int)(mx >> 7);
+          const int k = e == 255 || mx == 0 ? 0 : min(14 + 126 - e, 126);
+          const float up = __int_as_float((127 + k) << 23);
+          if (ch == 0) row_unscale[x * 128 + (warp & 3) * 32 + (i0 + i) * RPI + lane / LPR] = __int_as_float((127 - k) << 23);
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = unpack2<T>(u[q]);
+            u[q] = pack2<__half>(f.x * up, f.y * up);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sts16(q_at(i0 + i), v[i].x, v[i].y, v[i].z, v[i].w);
       }
     }
     proxy_fence();
     __syncwarp();
     if (lane == 0) arrive_lead<CG>(mbar::saddr(&q_full));
+    vf = p.cache.scales[p.cache.heads + it.h];
     const float unscale = std::is_same<T, __nv_bfloat16>::value ? row_unscale[x * 128 + rr] : 1.f;
     // score -> log2 units; not zero, so that a masked -inf stays -inf
     c = fmaxf(p.scale_log2 * unscale * p.cache.scales[it.h], 1.2e-38f);
@@ -655,7 +667,6 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   if (soft) {
     // ---- the row's output
     fence_after();
-    const float vf = p.cache.scales[p.cache.heads + it.h];
     uint32_t nan_groups = 0;
     if (nan_seen && real) {
       // rare: which groups of 16 channels see a value that is NaN

@@ -548,10 +548,10 @@ def test_attention_page_numbers_are_clamped(ext, cuda_device):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("q", [1, 140])
-def test_attention_other_stream_and_graph(ext, cuda_device, q):
+@pytest.mark.parametrize("q,hq,hkv", [(1, 8, 2), (140, 8, 2), (600, 64, 16)])
+def test_attention_other_stream_and_graph(ext, cuda_device, q, hq, hkv):
     c = {k: (v.to(cuda_device) if torch.is_tensor(v) else v) for k, v in
-         attention_case([(q, 900), (q, 150)], 8, 2, 128, 16, torch.float16).items()}
+         attention_case([(q, 900), (q, max(q, 150))], hq, hkv, 128, 16, torch.float16).items()}
     ref = run_attention(ext, cuda_device, c)
     out = torch.zeros_like(ref)
     st = torch.cuda.Stream()
@@ -647,6 +647,17 @@ def test_attention_one_prompt_among_single_tokens(ext, cuda_device, hq, hkv, d):
         run_attention(ext, cuda_device, dict(c, table=c["table"][part], seq=c["seq"][part],
                                              start=c["start"][part.start:part.stop + 1]), max_q=longest, out=out)
     assert ((out.cpu().double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("longest", [60, 900])
+def test_attention_more_requests_than_a_launch_takes(ext, cuda_device, longest):
+    gen = torch.Generator().manual_seed(9)
+    lens = [(0 if n % 7 == 0 else 1, n) for n in torch.randint(0, longest, (2500,), generator=gen).tolist()]
+    c = attention_case(lens, 4, 2, 64, 32, torch.float16)
+    got = run_attention(ext, cuda_device, c).cpu()
+    ref, vmax = attention_by_matrices(cuda_device, c, 0)
+    assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
 
 
 @pytest.mark.gpu
