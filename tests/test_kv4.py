@@ -684,3 +684,52 @@ def test_attention_many_rows_nan_stays_behind(ext, cuda_device, d):
         nan[1201 - (n - key):1201, 8:16, 16 * group:16 * group + 16] = True
     got = run_attention(ext, cuda_device, c).cpu()
     assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], ref[~nan])
+
+
+# ---- keys of a few row blocks split over the SMs and joined ---------------------------
+
+def split_case(hq, hkv, d, q, n, dt, page=64):
+    """A chunk behind a long context, one behind a short one, one whose first rows stand before position 0."""
+    return attention_case([(q, n), (q, n // 7), (q, 5)], hq, hkv, d, page, DT[dt])
+
+
+def check_is_split(c):
+    """Few row blocks against 148 SMs and 8 tiles and more: the pieces go through the workspace."""
+    assert cabi.lib().cek_kv4_attention_workspace_bytes(len(c["seq"]), c["q"].shape[0], c["q"].shape[1], c["cache"].shape[1],
+                                                        c["q"].shape[2], c["max_q"], c["max_seq"]) > 0
+
+
+SPLIT = [(8, 1, 128, 10, 4097), (8, 1, 128, 40, 5000), (8, 2, 128, 140, 900), (4, 2, 256, 40, 4097), (4, 1, 256, 130, 5003),
+         (4, 1, 64, 20, 4097), (8, 2, 64, 50, 6001)]  # one row block and two beside each other of each width
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,q,n", SPLIT)
+@pytest.mark.parametrize("window", [0, 100, 2500])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_attention_split_keys(ext, cuda_device, hq, hkv, d, q, n, window, dt):
+    """With a window most pieces hold no tile."""
+    c = split_case(hq, hkv, d, q, n, dt)
+    check_is_split(c)
+    got = run_attention(ext, cuda_device, c, window).cpu()
+    ref, vmax = attention_by_matrices(cuda_device, c, window)
+    ref = ref.nan_to_num()  # softmax over no keys
+    assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
+    assert not got[2 * q:3 * q - 5].any()
+    assert torch.equal(got, run_attention(ext, cuda_device, c, window).cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,q,n", SPLIT)
+def test_attention_split_keys_nan(ext, cuda_device, hq, hkv, d, q, n):
+    """NaN value scales: in a middle piece, for every row of a kv head, and near the end, for its last rows."""
+    c = split_case(hq, hkv, d, q, n, "f16")
+    check_is_split(c)
+    ref = run_attention(ext, cuda_device, c).cpu()
+    off, page, group, h = K.offsets(64, d), 64, hq // hkv, hkv - 1
+    nan = torch.zeros_like(ref, dtype=torch.bool)
+    for key, g16 in (((n - q) // 2, 1), (n - 3, d // 16 - 1)):
+        c["cache"][c["table"][0, key // page].item(), h, off[3] + (key % page) * (d // 16) + g16] = 0x7F
+        nan[max(0, key - (n - q)):q, h * group:(h + 1) * group, 16 * g16:16 * g16 + 16] = True
+    got = run_attention(ext, cuda_device, c).cpu()
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], ref[~nan])
