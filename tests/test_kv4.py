@@ -733,3 +733,67 @@ def test_attention_split_keys_nan(ext, cuda_device, hq, hkv, d, q, n):
         nan[max(0, key - (n - q)):q, h * group:(h + 1) * group, 16 * g16:16 * g16 + 16] = True
     got = run_attention(ext, cuda_device, c).cpu()
     assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], ref[~nan])
+
+
+# ---- append and gather on both sides of the change to two units a thread ----------------
+
+def units_of_32_blocks(dev, d, channels):
+    return 256 // (d // channels) * 32 * torch.cuda.get_device_properties(dev).multi_processor_count
+
+
+def near(dev, d, channels, hkv, more):
+    return units_of_32_blocks(dev, d, channels) // hkv + more
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,hkv,page,dt,aligned", [(64, 7, 16, "f16", True), (64, 32, 128, "bf16", False), (128, 8, 64, "bf16", True),
+                                                   (128, 5, 32, "f16", False), (256, 3, 16, "f16", True), (256, 32, 64, "bf16", False)])
+@pytest.mark.parametrize("more", [0, 1, 40])
+def test_append_bits_long(ext, cuda_device, d, hkv, page, dt, aligned, more):
+    """Tokens drawn from a pool whose codes the oracle gives; the last slots skipped, negative or past the cache."""
+    dev, pool = cuda_device, 512
+    T = near(dev, d, 16, hkv, more)
+    gen = torch.Generator().manual_seed(T)
+    scales = scales_for(hkv, gen)
+    k, v = (special((torch.randn(pool, hkv, d, generator=gen) * size).to(DT[dt])) for size in (1.0, 0.1))
+    pick = torch.randint(0, pool, (T,), generator=gen)
+    pages = -(-T // page) + 1
+    slots = torch.randperm(pages * page, generator=gen)[:T]
+    slots[-2], slots[-5], slots[T // 2] = -1, pages * page, -7
+    ref = torch.zeros(pages, hkv, page_bytes(page, d), dtype=torch.uint8)
+    off, ok = K.offsets(page, d), (slots >= 0) & (slots < pages * page)
+    p, r = slots[ok] // page, slots[ok] % page
+    for part, x in ((0, k), (1, v)):
+        for start, width, what in zip(off[2 * part:], (d // 2, d // 16), K.quantize(x, scales[part])):
+            ref[:, :, start:start + page * width].view(pages, hkv, page, width)[p, :, r] = what[pick[ok]]
+    lead = 0 if aligned else 1
+    wide = torch.zeros(T, hkv, d + 8, dtype=DT[dt], device=dev)
+    wide[:, :, lead:lead + d] = k.to(dev)[pick.to(dev)]
+    cache = torch.zeros_like(ref, device=dev)
+    ext.esimd_kv4_append(wide[:, :, lead:lead + d], v.to(dev)[pick.to(dev)], scales.to(dev), slots.to(dev), cache, page)
+    assert torch.equal(cache.cpu(), ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,hkv,page,dt,aligned", [(64, 32, 16, "bf16", True), (64, 7, 128, "f16", False), (128, 8, 64, "f16", True),
+                                                   (128, 5, 32, "bf16", False), (256, 3, 16, "bf16", True), (256, 32, 64, "f16", False)])
+@pytest.mark.parametrize("more", [0, 1, 40])
+def test_gather_long(ext, cuda_device, d, hkv, page, dt, aligned, more):
+    """Slots of a small cache read many times over; some near the end negative or past the cache."""
+    dev, pages = cuda_device, 5
+    T = near(dev, d, 8, hkv, more)
+    gen = torch.Generator().manual_seed(T)
+    scales = scales_for(hkv, gen)
+    cache = torch.randint(0, 256, (pages, hkv, page_bytes(page, d)), generator=gen, dtype=torch.uint8)
+    slots = torch.randint(0, pages * page, (T,), generator=gen)
+    slots[-1], slots[-4], slots[T // 2] = pages * page, -1, -9
+    ok = ((slots >= 0) & (slots < pages * page))[:, None, None]
+    lead = 0 if aligned else 1
+    wide = torch.full((2, T, hkv, d + 8), 7.0, dtype=DT[dt], device=dev)
+    out = wide[:, :, :, lead:lead + d]
+    ext.esimd_kv4_gather(cache.to(dev), scales.to(dev), slots.to(dev), out[0], out[1], page)
+    for part in (0, 1):
+        values = torch.from_numpy(K.decode(cache, page, d, torch.arange(pages * page).numpy(), part, scales)).float().to(DT[dt])
+        ref = torch.where(ok, values[slots.clamp(0, pages * page - 1)], torch.zeros((), dtype=DT[dt]))
+        assert torch.equal(torch.nan_to_num(out[part].cpu(), 1234.0), torch.nan_to_num(ref, 1234.0))
+    assert (wide[..., :lead] == 7).all() and (wide[..., lead + d:] == 7).all()
