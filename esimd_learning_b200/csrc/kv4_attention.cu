@@ -308,7 +308,7 @@ attn_decode_kernel(const AttnParams p) {
         const int c = s.rb * ROWS + nt * 8 + 2 * t + j;
         const int pos = s.r.pos0 + c / p.group;
         hi[nt][j] = c < rows ? min(pos + 1, s.r.end) : 0;
-        lo[nt][j] = p.window > 0 ? pos - p.window + 1 : 0;
+        lo[nt][j] = first_key(p, pos);
         if (c < rows) {
           all_hi = min(all_hi, hi[nt][j]);
           all_lo = max(all_lo, lo[nt][j]);

@@ -28,6 +28,12 @@ int64_t prefill_workspace(int64_t d, int64_t requests, int64_t tokens, int64_t h
 int prefill_launch(int dtype, int64_t d, const AttnParams& p, int64_t max_seq, cudaStream_t st);
 bool prefill_timeouts(unsigned long long* count);
 
+// First key that a row at position pos sees.  A row before position 0 sees none; with a window
+// near 2^31 its pos - window would leave 32 bits.
+CEK_DEVICE int first_key(const AttnParams& p, int pos) {
+  return p.window > 0 ? max(max(pos, -1) + 1 - p.window, 0) : 0;
+}
+
 // What a request asks for, from its lengths.
 struct Request {
   int t0, n;          // first token row, rows tokens (bounded)
@@ -45,8 +51,7 @@ CEK_DEVICE Request request_of(const AttnParams& p, int b) {
   r.n = min(n, p.max_q);
   r.pos0 = max(seq, 0) - n;  // a refused request (negative): every row stands before position 0
   r.end = max(0, min(min(r.pos0 + r.n, p.max_seq), p.key_limit));
-  const int lo = p.window > 0 ? max(0, r.pos0 - p.window + 1) : 0;
-  r.tile0 = min(lo, r.end) / TK;
+  r.tile0 = min(first_key(p, r.pos0), r.end) / TK;
   r.live = r.n > 0 ? max(1, (r.end + TK - 1) / TK - r.tile0) : 0;
   r.tiles = p.pad_tiles > 0 && r.n > 0 ? p.pad_tiles : r.live;
   return r;

@@ -254,7 +254,7 @@ CEK_DEVICE bool item_of(const AttnParams& p, int row_blocks, int splits, Item& i
   it.rows = it.r.n * p.group;
   if (it.rb * ROWS >= it.rows) return false;
   const int last = min(it.rows, (it.rb + 1) * ROWS) - 1;
-  const int lo = p.window > 0 ? max(0, it.r.pos0 + it.rb * ROWS / p.group - p.window + 1) : 0;
+  const int lo = first_key(p, it.r.pos0 + it.rb * ROWS / p.group);
   it.limit = min(it.r.pos0 + last / p.group + 1, it.r.end);
   const int t0 = lo / TK, n = it.limit > lo ? (it.limit + TK - 1) / TK - t0 : 0;
   const int a = (int)((int64_t)n * it.split / splits), z = (int)((int64_t)n * (it.split + 1) / splits);
@@ -313,7 +313,7 @@ attn_prefill_kernel(const AttnParams p, int row_blocks, int splits) {
   const int qi = row / p.group, tok = it.r.t0 + qi, head = it.h * p.group + row - qi * p.group;
   const bool real = soft && row < it.rows && tok >= 0 && tok < p.tokens;
   const int pos = it.r.pos0 + qi;
-  const int hi = row < it.rows ? min(pos + 1, it.r.end) : 0, lo = p.window > 0 ? pos - p.window + 1 : 0;
+  const int hi = row < it.rows ? min(pos + 1, it.r.end) : 0, lo = first_key(p, pos);
 
   constexpr int LPR = D / 8, RPI = 32 / LPR;  // lanes of a row of Q or of the output, rows at a time
   const int ch = lane % LPR;

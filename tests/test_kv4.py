@@ -797,3 +797,15 @@ def test_gather_long(ext, cuda_device, d, hkv, page, dt, aligned, more):
         ref = torch.where(ok, values[slots.clamp(0, pages * page - 1)], torch.zeros((), dtype=DT[dt]))
         assert torch.equal(torch.nan_to_num(out[part].cpu(), 1234.0), torch.nan_to_num(ref, 1234.0))
     assert (wide[..., :lead] == 7).all() and (wide[..., lead + d:] == 7).all()
+
+
+# ---- numbers at the end of 32 bits ------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hq,hkv,d,q,n", [(2, 1, 64, 300, 150), (8, 1, 128, 200, 190), (4, 1, 256, 100, 70), (8, 2, 128, 4, 2),
+                                          (1, 1, 64, 1, 9)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30])
+def test_attention_window_beyond_any_length(ext, cuda_device, hq, hkv, d, q, n, window):
+    """No window at all, also for a request whose first rows stand before position 0."""
+    c = attention_case([(q, n), (q, 900)], hq, hkv, d, 16, torch.float16)
+    assert torch.equal(run_attention(ext, cuda_device, c, window).cpu(), run_attention(ext, cuda_device, c).cpu())
