@@ -256,6 +256,7 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
   if (tid == 0) carry_q = carry_n = granted_pages = 0;
   const int avail = min(max(*free_count, 0), pool);
+  const int64_t row_tokens = min((int64_t)W * P.d, (int64_t)INT32_MAX);
   const int threads = blockDim.x, warps = threads >> 5;
   for (int b0 = 0; b0 < B; b0 += threads) {
     const int i = b0 + tid;
@@ -265,9 +266,9 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
       q = max(query_lens[i], 0);
       c = context_lens[i];
       if (c >= 0) {
-        const int have = pages_of(c, P), all = pages_of(c + q, P);
-        fits = all <= W;
-        need = fits ? all - have : 0;
+        // c + q may leave 32 bits; where it fits the row it does not
+        fits = (int64_t)c + q <= row_tokens;
+        need = fits ? pages_of(c + q, P) - pages_of(c, P) : 0;
       }
     }
     int sq = q, sn = need;  // inclusive scans
@@ -338,9 +339,10 @@ plan_kernel(const int32_t* __restrict__ query_lens, const int32_t* context_lens,
       slot[k] = -1;
       position[k] = 0;
       if (x[k] >= total || x[k] >= tokens) continue;
-      const int i = at[k], c = ctx[i], pos = (c < 0 ? ~c : c) + x[k] - start[i];
-      position[k] = pos;
+      const int i = at[k], c = ctx[i];
+      position[k] = (int64_t)(c < 0 ? ~c : c) + (x[k] - start[i]);
       if (c >= 0) {
+        const int pos = (int)position[k];
         const int have = pages_of(c, P), pg = (int)divide((uint32_t)pos, P);
         const int page = pg < have ? block_table[(int64_t)i * table_stride + pg] : free_pages[avail - 1 - (asked[i] + pg - have)];
         slot[k] = (int64_t)page * P.d + (pos - pg * (int)P.d);

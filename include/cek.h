@@ -357,7 +357,7 @@ CEK_API int64_t cek_kv4_page_bytes(int64_t page_size, int64_t head_dim);
  * A request that the stack (in order) or its table row cannot serve is refused
  * whole: it takes no page, its slots are -1 and its seq_lens entry is ~c_i
  * (negative), which attention reads as an empty request and a later plan
- * keeps refused.  Negative n count as 0.
+ * keeps refused; so is one whose c_i + n_i reaches 2^31.  Negative n count as 0.
  * seq_lens may be context_lens and free_count_out may be free_count (the state
  * then advances in place: nothing of them is written before all is read); no
  * other arrays may overlap.  The sums of n and of need must stay below 2^31.

@@ -809,3 +809,17 @@ def test_attention_window_beyond_any_length(ext, cuda_device, hq, hkv, d, q, n, 
     """No window at all, also for a request whose first rows stand before position 0."""
     c = attention_case([(q, n), (q, 900)], hq, hkv, d, 16, torch.float16)
     assert torch.equal(run_attention(ext, cuda_device, c, window).cpu(), run_attention(ext, cuda_device, c).cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [12, 16])
+@pytest.mark.parametrize("c,n", [(2 ** 31 - 1, 1_200_000_000), (2 ** 31 - 2, 3), (2 ** 31 - 1, 0), (5, 2 ** 31 - 50)])
+def test_plan_refuses_lengths_past_32_bits(ext, cuda_device, page, c, n):
+    """A sum that would wrap is refused like any that its row cannot hold; the requests beside it are served."""
+    got = run_plan(ext, cuda_device, [2, n, 1], [3, c, 5], [[7, 0], [0, 0], [8, 9]], [1, 2, 3], 3, page, 4)
+    first = [7 * page + 3, 7 * page + 4]
+    if n:
+        pos, slots = [3, 4, c, c + 1], first + [-1, -1]
+    else:
+        pos, slots = [3, 4, 5, 0], first + [8 * page + 5, -1]
+    assert got == ([[7, 0], [0, 0], [8, 9]], [0, 2, n + 2, n + 3], [5, ~c, 6], 3, pos, slots)
