@@ -60,7 +60,7 @@ cek_kv4_cache make_cache(const at::Tensor& kv_cache, const at::Tensor& kv_scales
   TORCH_CHECK(kv_scales.scalar_type() == at::kFloat && kv_scales.is_contiguous() && kv_scales.dim() == 2 &&
                   kv_scales.size(0) == 2 && kv_scales.size(1) == kv_cache.size(1),
               op, ": kv_scales must be contiguous fp32 [2, kv_heads]");
-  TORCH_CHECK(kv_cache.size(0) > 0, op, ": kv_cache must have at least one page");
+  TORCH_CHECK(kv_cache.size(0) > 0 && kv_cache.size(1) > 0, op, ": kv_cache must have at least one page and one kv head");
   cek_kv4_cache c;
   c.data = kv_cache.data_ptr();
   c.scales = kv_scales.data_ptr<float>();

@@ -823,3 +823,22 @@ def test_plan_refuses_lengths_past_32_bits(ext, cuda_device, page, c, n):
     else:
         pos, slots = [3, 4, 5, 0], first + [8 * page + 5, -1]
     assert got == ([[7, 0], [0, 0], [8, 9]], [0, 2, n + 2, n + 3], [5, ~c, 6], 3, pos, slots)
+
+
+# ---- a cache without heads ---------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [0, 4])
+def test_cache_without_heads_is_refused(ext, cuda_device, heads):
+    i32 = dict(dtype=torch.int32, device=cuda_device)
+    cache = torch.zeros(2, 0, page_bytes(16, 64), dtype=torch.uint8, device=cuda_device)
+    scales = torch.ones(2, 0, device=cuda_device)
+    q = torch.zeros(1, heads, 64, dtype=torch.float16, device=cuda_device)
+    with pytest.raises(RuntimeError):
+        ext.esimd_kv4_attention(q, cache, scales, torch.zeros(1, 1, **i32), torch.tensor([0, 1], **i32), torch.ones(1, **i32),
+                                torch.zeros_like(q), 16, 0.125, 1, 16)
+    kv, slots = q[:, :0], torch.zeros(1, dtype=torch.int64, device=cuda_device)
+    with pytest.raises(RuntimeError):
+        ext.esimd_kv4_append(kv, kv, scales, slots, cache, 16)
+    with pytest.raises(RuntimeError):
+        ext.esimd_kv4_gather(cache, scales, slots, kv, kv, 16)
