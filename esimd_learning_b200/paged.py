@@ -76,10 +76,11 @@ class PagedKV4Cache:
 
 
 class _Step:
-    """A captured decode step: write `hidden`, replay, read `output`.  Holds what the graph reads besides."""
+    """A captured decode step: write `hidden`, replay, read `output`.  Holds what the graph reads besides: the
+    lengths, and the model with its weights and cache."""
 
-    def __init__(self, hidden, query_lens, output, graph):
-        self.hidden, self.query_lens, self.output, self.graph = hidden, query_lens, output, graph
+    def __init__(self, hidden, query_lens, output, graph, model):
+        self.hidden, self.query_lens, self.output, self.graph, self.model = hidden, query_lens, output, graph, model
 
     def replay(self):
         self.graph.replay()
@@ -173,7 +174,7 @@ class PagedDecoder:
         with torch.cuda.stream(st), torch.cuda.graph(graph, stream=st):
             output = self._run(hidden, n, requests, 1)
         torch.cuda.current_stream(dev).wait_stream(st)
-        return _Step(hidden, n, output, graph)
+        return _Step(hidden, n, output, graph, self)
 
 
 def main() -> None:

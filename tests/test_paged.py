@@ -95,3 +95,19 @@ def test_refusal_and_release(ext, cuda_device):
     again = model.forward(hidden(60, 2, cuda_device)[:30], [30, 0, 0, 0])
     # other row counts take other GEMM tiles, but each row's arithmetic is its own
     torch.testing.assert_close(again, a[:30])
+
+
+@pytest.mark.gpu
+def test_captured_step_keeps_what_it_reads(ext, cuda_device):
+    """The step alone is enough: weights and cache live as long as it does."""
+    import gc
+    import weakref
+    model, cache = make(cuda_device, layers=1)
+    step = model.capture(2)
+    read = [weakref.ref(t) for t in (model.cos_sin, model.layers[0]["qkv"][0], cache.pages, cache.scales, cache.block_table,
+                                     cache.context_lens, cache.free_pages, cache.free_count)]
+    del model, cache
+    gc.collect()
+    assert all(r() is not None for r in read)
+    step.hidden.copy_(hidden(2, 0, cuda_device))
+    assert torch.isfinite(step.replay()).all()
