@@ -52,6 +52,8 @@ class PagedKV4Cache:
         nbytes = cabi.lib().cek_kv4_page_bytes(page_size, shape.head_dim)
         if nbytes == 0:
             raise ValueError(f"page_size {page_size} or head_dim {shape.head_dim} is not supported")
+        if max_seq_len > shape.max_position:  # RoPE would take the last position for all behind it
+            raise ValueError(f"max_seq_len {max_seq_len} is beyond the {shape.max_position} positions of the shape")
         i32 = dict(dtype=torch.int32, device=device)
         self.pages = torch.empty(layers, num_pages, shape.num_kv_heads, nbytes, dtype=torch.uint8, device=device)
         self.scales = torch.ones(layers, 2, shape.num_kv_heads, dtype=torch.float32, device=device)

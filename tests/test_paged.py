@@ -111,3 +111,11 @@ def test_captured_step_keeps_what_it_reads(ext, cuda_device):
     assert all(r() is not None for r in read)
     step.hidden.copy_(hidden(2, 0, cuda_device))
     assert torch.isfinite(step.replay()).all()
+
+
+def test_refuses_lengths_without_positions():
+    """Positions past the RoPE table would all turn like its last one."""
+    from esimd_learning_b200.paged import PagedKV4Cache
+    assert PagedKV4Cache(1, SHAPE, 4, 1, SHAPE.max_position, "cpu").block_table.shape == (1, SHAPE.max_position // 64)
+    with pytest.raises(ValueError):
+        PagedKV4Cache(1, SHAPE, 4, 1, SHAPE.max_position + 1, "cpu")
