@@ -23,6 +23,8 @@ a captured decode step needs no host work between replays.
 """
 from __future__ import annotations
 
+import dataclasses
+
 import torch
 
 from esimd_learning_b200.chain import ChainShape, SMALL, _quantize_rows, full_weights, rope_cache
@@ -42,22 +44,25 @@ class PagedKV4Cache:
     pages: uint8 [layers, num_pages, kv_heads, page bytes]; one page number
     serves all layers.  scales: fp32 [layers, 2, kv_heads] (keys, values), to be
     calibrated; 1.0 keeps values between 2^-10 and 2688.  block_table,
-    context_lens, free_pages and free_count are the planner's state."""
+    context_lens, free_pages and free_count are the planner's state.  Requests
+    end at whole pages: max_seq_len is rounded up to one."""
 
     def __init__(self, layers: int, shape: ChainShape, num_pages: int, max_requests: int, max_seq_len: int, device,
                  page_size: int = 64):
         from esimd_learning_b200 import cabi
 
-        self.page_size, self.max_seq_len, self.max_requests, self.device = page_size, max_seq_len, max_requests, device
+        self.page_size, self.max_requests, self.device = page_size, max_requests, device
         nbytes = cabi.lib().cek_kv4_page_bytes(page_size, shape.head_dim)
         if nbytes == 0:
             raise ValueError(f"page_size {page_size} or head_dim {shape.head_dim} is not supported")
         if max_seq_len > shape.max_position:  # RoPE would take the last position for all behind it
             raise ValueError(f"max_seq_len {max_seq_len} is beyond the {shape.max_position} positions of the shape")
+        width = -(-max_seq_len // page_size)
+        self.max_seq_len = width * page_size  # what the planner grants a row, and attention's bound
         i32 = dict(dtype=torch.int32, device=device)
         self.pages = torch.empty(layers, num_pages, shape.num_kv_heads, nbytes, dtype=torch.uint8, device=device)
         self.scales = torch.ones(layers, 2, shape.num_kv_heads, dtype=torch.float32, device=device)
-        self.block_table = torch.zeros(max_requests, -(-max_seq_len // page_size), **i32)
+        self.block_table = torch.zeros(max_requests, width, **i32)
         self.context_lens = torch.zeros(max_requests, **i32)
         self.free_pages = torch.arange(num_pages, **i32)
         self.free_count = torch.tensor([num_pages], **i32)
@@ -99,7 +104,8 @@ class PagedDecoder:
         self.ops, self.shape, self.cache, self.window = ops, shape, cache, window
         dev = cache.device
         self.layers = [{k: tuple(t.to(dev) for t in v) if isinstance(v, tuple) else v.to(dev) for k, v in w.items()} for w in layers]
-        self.cos_sin = rope_cache(shape, dev)
+        # the cache's last page may reach past the shape's positions
+        self.cos_sin = rope_cache(dataclasses.replace(shape, max_position=max(shape.max_position, cache.max_seq_len)), dev)
 
     def _project(self, x, weight, scale):
         """x [T, K] @ weight^T: the GEMV family up to 16 tokens, per-token FP8 on the tensor cores above."""

@@ -119,3 +119,17 @@ def test_refuses_lengths_without_positions():
     assert PagedKV4Cache(1, SHAPE, 4, 1, SHAPE.max_position, "cpu").block_table.shape == (1, SHAPE.max_position // 64)
     with pytest.raises(ValueError):
         PagedKV4Cache(1, SHAPE, 4, 1, SHAPE.max_position + 1, "cpu")
+
+
+@pytest.mark.gpu
+def test_lengths_up_to_the_last_page(ext, cuda_device):
+    """max_seq_len inside a page: the planner hands that page out whole, and attention reads all of it."""
+    model, cache = make(cuda_device, num_pages=34, requests=2, max_seq=SHAPE.max_position - 6)
+    for step, n in enumerate([[480, 3], [24, 1], [7, 0], [1, 1]]):
+        out = model.forward(hidden(sum(n), step, cuda_device), n)
+        assert torch.isfinite(out).all()
+        check_last_layer(model, cache, 1)
+    assert cache.context_lens.tolist() == [512, 5]
+    assert cache.max_seq_len == 512 and model.cos_sin.shape[0] >= 512
+    model.forward(hidden(1, 9, cuda_device), [1, 0])
+    assert cache.refused() == [0]
