@@ -785,8 +785,11 @@ using namespace cek::kv4;
 // not fit its registers: 16 rows on 500 keys 21.5 us against 16.4.
 inline int64_t decode_rows(int64_t d) { return d == 256 ? 8 : 32; }
 
+// Keys of a request and rows of its kv head: 32-bit numbers with room for a tile or a row block behind them.
+constexpr int64_t kMaxKeys = INT32_MAX - 127, kMaxRows = INT32_MAX - 1023;
+
 struct DecodePlan {
-  int nt, ctas;
+  int nt, tile_keys, ctas;
   int pad;              // tiles of a segment where all are short, else 0
   size_t smem;
   bool join;            // some segment may be in several pieces
@@ -798,6 +801,7 @@ DecodePlan plan_decode_dn(int64_t requests, int64_t heads, int64_t group, int64_
   using C = DecodeCfg<D, NT>;
   DecodePlan d;
   d.nt = NT;
+  d.tile_keys = C::TK;
   const int64_t req = std::min<int64_t>(requests, kMaxRequests);
   const int64_t segments = req * heads * ((max_q * group + 8 * NT - 1) / (8 * NT));
   const int64_t tiles = std::max<int64_t>(1, (max_seq + C::TK - 1) / C::TK);
@@ -822,6 +826,15 @@ DecodePlan plan_decode(int64_t d, int64_t requests, int64_t heads, int64_t group
   return d == 64    ? plan_decode_d<64>(requests, heads, group, max_q, max_seq)
          : d == 128 ? plan_decode_d<128>(requests, heads, group, max_q, max_seq)
                     : plan_decode_d<256>(requests, heads, group, max_q, max_seq);
+}
+
+// Requests of one launch: their prefix sums sit in shared memory, and the line of their tiles
+// is counted in 32 bits with room for a product by the warps of a CTA.  0: one has too many tiles.
+int64_t decode_requests(const AttnParams& p, const DecodePlan& d) {
+  const int64_t keys = std::min(p.max_seq, p.key_limit);
+  const int64_t tiles = std::max<int64_t>(std::max(1, d.pad), (keys + d.tile_keys - 1) / d.tile_keys);
+  const int64_t blocks = ((int64_t)p.max_q * p.group + 8 * d.nt - 1) / (8 * d.nt);
+  return std::min<int64_t>(kMaxRequests, INT32_MAX / kDecodeWarps / (tiles * p.cache.heads * blocks));
 }
 
 template <typename T, int D, int NT>
@@ -865,10 +878,11 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
   if (s != CEK_OK) return s;
   if (dtype != CEK_F16 && dtype != CEK_BF16) return CEK_ERR_INVALID_ARG;
   if (requests < 0 || requests > 65535 || tokens < 0 || tokens > INT32_MAX || q_heads <= 0 ||
-      q_heads % cache->kv_heads || q_heads > 65535 || table_width < 0 || table_width * cache->page_size > INT32_MAX ||
+      q_heads % cache->kv_heads || q_heads > 65535 || table_width < 0 || table_width > kMaxKeys / cache->page_size ||
       table_stride < table_width || max_query_len < 0 || max_seq_len < 0 || max_query_len > INT32_MAX ||
       max_seq_len > INT32_MAX || window < 0 || window > INT32_MAX)
     return CEK_ERR_INVALID_ARG;
+  if (std::min(max_query_len, tokens) * (q_heads / cache->kv_heads) > kMaxRows) return CEK_ERR_INVALID_ARG;
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return CEK_ERR_INVALID_ARG;
   if (requests == 0 || tokens == 0 || max_query_len == 0) return CEK_OK;
   if (!query || !out || !query_start || !seq_lens || (table_width > 0 && !block_table)) return CEK_ERR_INVALID_ARG;
@@ -905,9 +919,11 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
     if (d.partial_bytes > 0 && !cek_host::aligned16(workspace)) return CEK_ERR_ALIGNMENT;
     p.partial = d.join ? static_cast<float*>(workspace) : nullptr;
     p.pad_tiles = d.pad;
+    const int64_t part = decode_requests(p, d);
+    if (part == 0) return CEK_ERR_INVALID_ARG;
     int rc = CEK_OK;
-    for (int64_t b = 0; b < requests && rc == CEK_OK; b += kMaxRequests) {  // the prefix sums of a launch are bounded
-      p.requests = (int)std::min<int64_t>(kMaxRequests, requests - b);
+    for (int64_t b = 0; b < requests && rc == CEK_OK; b += part) {
+      p.requests = (int)std::min(part, requests - b);
       p.table = block_table + b * table_stride;
       p.query_start = query_start + b;
       p.seq_lens = seq_lens + b;

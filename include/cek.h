@@ -409,6 +409,9 @@ CEK_API int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, voi
  * host (a longer request is read as if cut there: its rows past the bound are
  * not written, its keys past it not read); seq_lens are also cut to
  * table_width * P.  Page numbers outside the cache are clamped into it.
+ * At most 65535 requests and heads; table_width * P and the rows of a kv head
+ * stay below 2^31 by a tile, and so do, for calls of few rows, four times the
+ * tiles (64 keys) of one request's heads: CEK_ERR_INVALID_ARG beyond.
  * A step that mixes single tokens with prompts is right in one call, but the
  * prompts' kernel then takes all of it: two calls with slices of the request
  * arrays (query_start holds rows of the whole query) give each its own.

@@ -842,3 +842,32 @@ def test_cache_without_heads_is_refused(ext, cuda_device, heads):
         ext.esimd_kv4_append(kv, kv, scales, slots, cache, 16)
     with pytest.raises(RuntimeError):
         ext.esimd_kv4_gather(cache, scales, slots, kv, kv, 16)
+
+
+# ---- counts at the end of 32 bits ----------------------------------------------------------
+
+@pytest.mark.parametrize("kw", [dict(W=2 ** 27, ts=2 ** 27), dict(W=2 ** 60, ts=2 ** 60), dict(T=2 ** 31 - 1, mq=2 ** 31 - 1),
+                                dict(T=2 ** 30, mq=2 ** 30, hq=8)])
+def test_attention_refuses_counts_past_32_bits(kw):
+    """Keys of a row of the table, rows of a kv head."""
+    assert _attend(**{"ms": 2 ** 31 - 1, **kw}) == cabi.CEK_ERR_INVALID_ARG
+
+
+def test_attention_refuses_more_tiles_than_it_counts():
+    """65535 heads over 2^27 keys: 2^37 tiles of one request."""
+    wide = dict(kv_heads=65535, page_stride=65535 * page_bytes(16, 64))
+    assert _attend(_cache(**wide), hq=65535, W=2 ** 23, ts=2 ** 23, ms=2 ** 27) == cabi.CEK_ERR_INVALID_ARG
+    assert _attend(_cache(**wide), hq=65535, B=0) == cabi.CEK_OK
+
+
+@pytest.mark.gpu
+def test_attention_loose_bounds_in_several_launches(ext, cuda_device):
+    """Tables so wide that the bound on tiles allows some 250 requests a launch; the lengths are short."""
+    gen = torch.Generator().manual_seed(11)
+    lens = [(0 if n % 7 == 0 else 1, n) for n in torch.randint(0, 700, (300,), generator=gen).tolist()]
+    c = attention_case(lens, 16, 8, 64, 128, torch.float16)
+    ref, vmax = attention_by_matrices(cuda_device, c, 0)
+    table = torch.zeros(300, 130000, dtype=torch.int32, device=cuda_device)
+    table[:, :c["table"].shape[1]] = c["table"].to(cuda_device)
+    got = run_attention(ext, cuda_device, dict(c, table=table), max_seq=130000 * 128).cpu()
+    assert ((got.double() - ref).abs() <= tolerance(ref, vmax, got.dtype)).all()
