@@ -903,9 +903,7 @@ extern "C" int cek_kv4_attention(const void* query, const cek_kv4_cache* cache, 
   p.ohs = out_head_stride;
   p.requests = (int)requests;
   p.tokens = (int)tokens;
-  p.q_heads = (int)q_heads;
   p.group = (int)(q_heads / cache->kv_heads);
-  p.table_width = (int)table_width;
   p.P = (int)cache->page_size;
   while ((1 << p.page_shift) < p.P) ++p.page_shift;
   p.max_q = (int)std::min(max_query_len, tokens);

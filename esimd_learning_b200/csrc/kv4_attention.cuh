@@ -15,8 +15,8 @@ struct AttnParams {
   const int32_t* query_start;
   const int32_t* seq_lens;
   int64_t table_stride, qts, qhs, ots, ohs;
-  int requests, tokens, q_heads, group, table_width, P, page_shift;  // P = 1 << page_shift
-  int max_q, max_seq, key_limit, window;  // key_limit: table_width * P
+  int requests, tokens, group, P, page_shift;  // P = 1 << page_shift
+  int max_q, max_seq, key_limit, window;  // key_limit: keys of a table row
   float scale_log2;  // softmax_scale * log2(e)
   float* partial;    // pieces of split segments
   int pad_tiles;     // decode: tiles that every request counts, 0: its own
