@@ -18,7 +18,7 @@ namespace kv4 {
 // every access of a warp is contiguous, and a unit's place is worked out once.
 // An append thread takes a whole group of 16, so that the scale is worked out
 // once.  Long calls give a thread U = 2 units, their loads in flight together;
-// short ones one, for more threads.
+// short ones one, for more threads (kManyAppend, kManyGather).
 // 32 769 tokens of 8 heads of 128 read back: 32 us, 5.4 TB/s (83 % of a copy; with
 // integer divisions by page and head count it was 41).  8191 tokens written:
 // 12.5 us, 3.4 TB/s, bound by the instructions of the quotients (20 us with a
@@ -437,8 +437,16 @@ int token_args(const void* key, const void* value, const int64_t* slots, const c
 }
 }  // namespace
 
+// Blocks an SM (of one unit a thread) above which a thread takes two.  Device time, one and
+// two units, 8 heads of 128 (64 and 256 channels turn within a step of the same place):
+//   blocks an SM      4           8           16          32          64          128
+//   append, us    5.1 / 4.6   6.9 / 7.6  11.4 / 12.4  20.9 / 21.5  39.7 / 39.8  76.9 / 76.0
+//   gather, us    2.7 / 2.8   3.7 / 3.6   6.8 / 6.5   12.1 / 11.2  22.3 / 19.6  42.4 / 36.5
+// An append thread has work enough of its own between its loads; a gather thread has not.
+constexpr int64_t kManyAppend = 64, kManyGather = 8;
+
 // Launches KERNEL on [tokens], in parts whose unit numbers stay below 2^31.
-#define CEK_KV4_DISPATCH(KERNEL, CHANNELS, A0, A1, A2, A3)                                                                    \
+#define CEK_KV4_DISPATCH(KERNEL, CHANNELS, MANY, A0, A1, A2, A3)                                                     \
   do {                                                                                                               \
     const int64_t per = 256 / (cache->head_dim / CHANNELS), row = cache->kv_heads;                                      \
     cudaStream_t st = static_cast<cudaStream_t>(stream);                                                             \
@@ -451,9 +459,7 @@ int token_args(const void* key, const void* value, const int64_t* slots, const c
     int rc = CEK_OK;                                                                                                 \
     for (int64_t t0 = 0; t0 < tokens && rc == CEK_OK; t0 += part) {                                                  \
       const uint32_t units = (uint32_t)(std::min(part, tokens - t0) * row);                                          \
-      /* one unit a thread until there are 32 blocks an SM (8191 tokens written and read: 19.2 us,   */              \
-      /* 19.6 with two), then two (32 769 tokens read back: 32.8 us, 37.3 with one)                  */              \
-      const bool many = units > per * 32 * cek_host::sm_count();                                                     \
+      const bool many = units > per * MANY * cek_host::sm_count();                                                   \
       const dim3 grid((unsigned)((units + per * (many ? 2 : 1) - 1) / (per * (many ? 2 : 1)))), block(256);          \
       auto go = [&](auto tag, auto dim, auto v) {                                                                    \
         using T = decltype(tag);                                                                                     \
@@ -488,7 +494,7 @@ extern "C" int cek_kv4_append(const void* key, const void* value, const int64_t*
   const int s = token_args(key, value, slot_mapping, cache, tokens, dtype, &done);
   if (done) return s;
   const cek::kv4::Cache c = cek_host::kv4_cache(cache);
-  CEK_KV4_DISPATCH(append_kernel, 16, static_cast<const T*>(key) + t0 * key_token_stride,
+  CEK_KV4_DISPATCH(append_kernel, 16, kManyAppend, static_cast<const T*>(key) + t0 * key_token_stride,
                    static_cast<const T*>(value) + t0 * value_token_stride, slot_mapping + t0, c);
 }
 
@@ -499,6 +505,6 @@ extern "C" int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, 
   const int s = token_args(key, value, slots, cache, tokens, dtype, &done);
   if (done) return s;
   const cek::kv4::Cache c = cek_host::kv4_cache(cache);
-  CEK_KV4_DISPATCH(gather_kernel, 8, c, slots + t0, static_cast<T*>(key) + t0 * key_token_stride,
+  CEK_KV4_DISPATCH(gather_kernel, 8, kManyGather, c, slots + t0, static_cast<T*>(key) + t0 * key_token_stride,
                    static_cast<T*>(value) + t0 * value_token_stride);
 }

@@ -737,12 +737,9 @@ def test_attention_split_keys_nan(ext, cuda_device, hq, hkv, d, q, n):
 
 # ---- append and gather on both sides of the change to two units a thread ----------------
 
-def units_of_32_blocks(dev, d, channels):
-    return 256 // (d // channels) * 32 * torch.cuda.get_device_properties(dev).multi_processor_count
-
-
-def near(dev, d, channels, hkv, more):
-    return units_of_32_blocks(dev, d, channels) // hkv + more
+def near(dev, d, channels, blocks, hkv, more):
+    """Tokens that fill `blocks` blocks an SM, the change's place, and `more`."""
+    return 256 // (d // channels) * blocks * torch.cuda.get_device_properties(dev).multi_processor_count // hkv + more
 
 
 @pytest.mark.gpu
@@ -752,7 +749,7 @@ def near(dev, d, channels, hkv, more):
 def test_append_bits_long(ext, cuda_device, d, hkv, page, dt, aligned, more):
     """Tokens drawn from a pool whose codes the oracle gives; the last slots skipped, negative or past the cache."""
     dev, pool = cuda_device, 512
-    T = near(dev, d, 16, hkv, more)
+    T = near(dev, d, 16, 64, hkv, more)
     gen = torch.Generator().manual_seed(T)
     scales = scales_for(hkv, gen)
     k, v = (special((torch.randn(pool, hkv, d, generator=gen) * size).to(DT[dt])) for size in (1.0, 0.1))
@@ -781,7 +778,7 @@ def test_append_bits_long(ext, cuda_device, d, hkv, page, dt, aligned, more):
 def test_gather_long(ext, cuda_device, d, hkv, page, dt, aligned, more):
     """Slots of a small cache read many times over; some near the end negative or past the cache."""
     dev, pages = cuda_device, 5
-    T = near(dev, d, 8, hkv, more)
+    T = near(dev, d, 8, 8, hkv, more)
     gen = torch.Generator().manual_seed(T)
     scales = scales_for(hkv, gen)
     cache = torch.randint(0, 256, (pages, hkv, page_bytes(page, d)), generator=gen, dtype=torch.uint8)
