@@ -37,18 +37,21 @@ namespace kv4 {
 //    then the value lanes of one access read four neighbouring keys.
 //  * The probabilities of a tile, rounded to fp16, turn into the second
 //    product's operand by movmatrix.  They are held as 2^kShift p, so that fp16
-//    keeps full precision down to p = 2^-28.
+//    keeps full precision down to p = 2^-28.  fp16 because a matrix operand has 16
+//    bits and this type the most of them; the sum of the probabilities is fp32.
 //  * bf16 queries are scaled by a power of two a row, exactly, into fp16's
 //    range: one multiply path for both types (what falls out below is 2^-38 of
 //    the row's largest channel).
 //
-// Bound: the conversion.  A tile of 64 keys of 128 channels takes ~2300
-// scheduler cycles (256 conversions at 2.3 cycles and more beside other integer
-// work, 256 scalings, 64 matrix instructions at 8.5), where HBM would deliver it
-// in 1580; more warps or shorter chains of products do not change it, fewer
-// integer instructions do.  131 071 keys of 64/8 heads of 128, one token: 47 us,
+// Bound: latency.  A tile of 64 keys of 128 channels is ~1180 instructions of a
+// scheduler (256 conversions, 256 scalings and 64 matrix instructions among them)
+// and takes it ~2300 cycles, where HBM would deliver it in 1580.  No pipe is full
+// (issue slots 50 %, ALU 44 %, tensor 19 %, DRAM 44 %): three warps a scheduler, what
+// the registers allow, mostly wait for their own last instruction.  More warps on
+// tiles of 32 keys or two accumulators for S did not help, fewer integer
+// instructions did.  131 071 keys of 64/8 heads of 128, one token: 47 us,
 // 3.2 TB/s with start and join (4.6 TB/s in between); 64 ragged requests to 8192
-// keys: 86 us, 3.9 TB/s; 17 keys: 6 us.
+// keys: 88 us, 3.8 TB/s; 17 keys: 6 us.
 constexpr float kShift = 14.f;
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
@@ -808,6 +811,7 @@ DecodePlan plan_decode_dn(int64_t requests, int64_t heads, int64_t group, int64_
   d.smem = (size_t)C::RING + sizeof(int32_t) * (req + 1);
   const int per_sm = (int)std::min<int64_t>(C::PER_SM, 233472 / (d.smem + 1024 + 512));  // 228 KB an SM, 1 KB a CTA reserved
   const int64_t most = (int64_t)std::max(1, per_sm) * cek_host::sm_count();
+  // (A window is not counted: its few tiles behind a long bound are cut all the same.)
   // A cut costs a second launch, 4 to 5 us: with a CTA for every segment, two tiles a warp
   // (another 1.3 us) are cheaper; otherwise a warp takes whole segments of up to four.
   d.pad = tiles <= (segments <= most ? 2 : 1) * kDecodeWarps ? (int)tiles : 0;

@@ -19,9 +19,9 @@ namespace kv4 {
 // An append thread takes a whole group of 16, so that the scale is worked out
 // once.  Long calls give a thread U = 2 units, their loads in flight together;
 // short ones one, for more threads (kManyAppend, kManyGather).
-// 32 769 tokens of 8 heads of 128 read back: 32 us, 5.4 TB/s (83 % of a copy; with
-// integer divisions by page and head count it was 41).  8191 tokens written:
-// 12.5 us, 3.4 TB/s, bound by the instructions of the quotients (20 us with a
+// 32 769 tokens of 8 heads of 128 read back: 32.2 us, 5.4 TB/s (82 % of a copy; with
+// integer divisions by page and head count it was 41).  8191 tokens written: 10.2 us,
+// 4.2 TB/s; 65 % of the issue slots are taken, most by the quotients (20 us with a
 // division a channel).
 template <typename T, bool VEC>
 CEK_DEVICE uint4 load8(const T* p) {

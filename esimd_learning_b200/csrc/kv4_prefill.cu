@@ -28,8 +28,8 @@
 // 2048 of exp2 (16 a cycle) and, in a pair, ~1500 of shared memory.  It takes
 // ~3500: a row block's softmax (2000) and its products (1024) follow each other,
 // and each hand-over costs a few hundred cycles; two row blocks hide a part of it.
-// 8192 tokens of 64/8 heads of 128 from an empty cache: 1078 us, 1020 TFLOP/s.  Six
-// ragged chunks of 16/4 heads of 256 with a window of 1024: 148 us, 553 TFLOP/s;
+// 8192 tokens of 64/8 heads of 128 from an empty cache: 1085 us, 1010 TFLOP/s.  Six
+// ragged chunks of 16/4 heads of 256 with a window of 1024: 147 us, 557 TFLOP/s;
 // there an item starts for 6 us and ends for 3 of its 27.
 //
 // The output is rescaled only when a row's maximum has grown by more than
@@ -807,7 +807,8 @@ inline Plan plan_of(int64_t d, int64_t requests, int64_t tokens, int64_t heads, 
   bool packed;
   r.cg = r.splits = 1;
   r.items = count(128 * r.nq, &packed);
-  // too few row blocks for the SMs: split their keys, at least four tiles a piece
+  // too few row blocks for the SMs: split their keys, at least four tiles of the longest bound a
+  // piece (behind a window most pieces have none: their blocks write an empty piece)
   const int64_t tiles = (max_seq + (d == 256 ? 63 : 127)) / (d == 256 ? 64 : 128);
   if (!packed && r.items < cek_host::sm_count() && tiles >= 8)
     r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(cek_host::sm_count() / r.items, tiles / 4));

@@ -414,7 +414,8 @@ CEK_API int cek_kv4_gather(const cek_kv4_cache* cache, const int64_t* slots, voi
  * tiles (64 keys) of one request's heads: CEK_ERR_INVALID_ARG beyond.
  * A step that mixes single tokens with prompts is right in one call, but the
  * prompts' kernel then takes all of it: two calls with slices of the request
- * arrays (query_start holds rows of the whole query) give each its own.
+ * arrays (query_start holds rows of the whole query) give each its own (a
+ * 512-token chunk beside 63 tokens behind 4000 keys each: 568 us, 130 in two).
  * workspace: cek_kv4_attention_workspace_bytes() bytes, 16-byte aligned,
  * contents ignored; may be null where that is 0.  One call at a time per
  * workspace.  Deterministic: no atomics order a sum. */
