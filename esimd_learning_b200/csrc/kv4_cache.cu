@@ -443,6 +443,7 @@ int token_args(const void* key, const void* value, const int64_t* slots, const c
 //   append, us    5.1 / 4.6   6.9 / 7.6  11.4 / 12.4  20.9 / 21.5  39.7 / 39.8  76.9 / 76.0
 //   gather, us    2.7 / 2.8   3.7 / 3.6   6.8 / 6.5   12.1 / 11.2  22.3 / 19.6  42.4 / 36.5
 // An append thread has work enough of its own between its loads; a gather thread has not.
+// (Append's half microsecond at 4 blocks, gone at 8, is not worth a second turn.)
 constexpr int64_t kManyAppend = 64, kManyGather = 8;
 
 // Launches KERNEL on [tokens], in parts whose unit numbers stay below 2^31.
